@@ -119,6 +119,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dsv4moe_shared_fp8_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "dsv4moe_shared_fp8_add": (ctypes.c_int, [_p, _i64, _i32, _i32, _p, _p, _p, _p, ctypes.c_float, _p, _p, _sz,
                                               _p]),
+    "dsv4moe_act_quant_int8": (ctypes.c_int, [_p, _i32, _i64, _i64, _p, _p, _p]),
+    "dsv4moe_int8_gemm": (ctypes.c_int, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p]),
+    "dsv4moe_int8_linear": (ctypes.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
+    "dsv4moe_grouped_gemm": (
+        ctypes.c_int,
+        [_p, _i64, _i32, _i32, _i64, _i64, _i32, _p, _p, _i64, _p, _p, _i32, _i32, _f32, _p, _p, _p],
+    ),
+    "dsv4moe_grouped_int8_gemm": (
+        ctypes.c_int,
+        [_p, _p, _i64, _i32, _i32, _i64, _i64, _i32, _p, _p, _p, _i64, _p, _p, _i32, _i32, _f32, _p, _p, _p],
+    ),
+    "dsv4moe_grouped_int8_linear": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i32, _i32, _i64, _i64, _i32, _p, _p, _p, _i64, _p, _p, _i32, _i32, _f32, _p, _p, _p, _p,
+         _p],
+    ),
 }
 
 _lock = threading.Lock()

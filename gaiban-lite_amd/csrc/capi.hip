@@ -9,6 +9,7 @@
 
 #include "act_quant.h"
 #include "common.h"
+#include "product_tile.h"
 #include "../../include/dsv4moe.h"
 
 namespace dsv4host {
@@ -65,6 +66,10 @@ static void prof_release() {
 }  // namespace dsv4host
 
 // kernel launchers (one per translation unit)
+int dsv4_launch_act_quant_int8(const void*, int32_t, int64_t, int64_t, int8_t*, float*, hipStream_t);
+int dsv4_launch_int8_gemm(const int8_t*, const float*, int64_t, int64_t, int64_t, const int8_t*, const uint16_t*,
+                          uint16_t*, hipStream_t);
+int dsv4_launch_grouped(const dsv4::ProductParams&, bool, bool, hipStream_t);
 int dsv4_launch_route_topk(const float*, const float*, int64_t, int32_t, int32_t, int32_t, float,
                            int32_t*, float*, float*, int32_t*, float*, hipStream_t);
 int dsv4_launch_route_hash(const float*, const int64_t*, int64_t, const int64_t*, int64_t, int32_t,
@@ -905,6 +910,162 @@ int dsv4moe_w8a16_fp8_linear(const uint16_t* a, int64_t m, int64_t n, int64_t k,
   DSV4_REQUIRE(k <= 32768, "w8a16_fp8_linear: k must be <= 32768, got %lld", (long long)k);
   return dsv4_launch_w8a16(a, m, n, k, wq, nullptr, ws8, split_k, workspace, out,
                            static_cast<hipStream_t>(stream), 0, weight_layout == DSV4MOE_WEIGHT_ROWMAJOR);
+}
+
+static int validate_act_quant_int8(const char* who, const void* x, int32_t x_dtype, int64_t m, int64_t k,
+                                   const int8_t* q, const float* scale) {
+  DSV4_REQUIRE(x_dtype >= 0 && x_dtype <= 2, "%s: x_dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)", who);
+  DSV4_REQUIRE(m >= 0 && m < (int64_t)1 << 31, "%s: m must be in [0, 2^31)", who);
+  DSV4_REQUIRE(k > 0 && k % 16 == 0 && k <= 65536, "%s: k must be a multiple of 16 in [16, 65536], got %lld", who,
+               (long long)k);
+  if (m == 0) return DSV4MOE_OK;
+  DSV4_REQUIRE(x && q && scale, "%s: null pointer", who);
+  DSV4_REQUIRE(aligned(x, 16) && aligned(q, 16), "%s: x and q must be 16-byte aligned", who);
+  return DSV4MOE_OK;
+}
+
+static int validate_int8_gemm(const char* who, const void* a, const float* a_scale, int64_t m, int64_t n, int64_t k,
+                              const int8_t* wq, const uint16_t* ws, const uint16_t* out) {
+  DSV4_REQUIRE(m >= 0 && m < (int64_t)1 << 31, "%s: m must be in [0, 2^31)", who);
+  DSV4_REQUIRE(n > 0 && n % 16 == 0, "%s: n must be a positive multiple of 16, got %lld", who, (long long)n);
+  DSV4_REQUIRE(k > 0 && k % 16 == 0 && k <= 65536, "%s: k must be a multiple of 16 in [16, 65536], got %lld", who,
+               (long long)k);
+  DSV4_REQUIRE(n < (int64_t)1 << 31 && n * k < (int64_t)1 << 31, "%s: n * k must be below 2^31", who);
+  DSV4_REQUIRE((m + 15) / 16 * (n / 16) < (int64_t)1 << 31, "%s: m * n too large", who);
+  if (m == 0) return DSV4MOE_OK;
+  DSV4_REQUIRE(a && a_scale && wq && ws && out, "%s: null pointer", who);
+  DSV4_REQUIRE(aligned(a, 16) && aligned(wq, 16) && aligned(ws, 16) && aligned(out, 16),
+               "%s: activation, weight, ws and out must be 16-byte aligned", who);
+  return DSV4MOE_OK;
+}
+
+int dsv4moe_act_quant_int8(const void* x, int32_t x_dtype, int64_t m, int64_t k, int8_t* q, float* scale,
+                           void* stream) {
+  clear_error();
+  const int rc = validate_act_quant_int8("act_quant_int8", x, x_dtype, m, k, q, scale);
+  if (rc != DSV4MOE_OK || m == 0) return rc;
+  return dsv4_launch_act_quant_int8(x, x_dtype, m, k, q, scale, static_cast<hipStream_t>(stream));
+}
+
+int dsv4moe_int8_gemm(const int8_t* a, const float* a_scale, int64_t m, int64_t n, int64_t k, const int8_t* wq,
+                      const uint16_t* ws, uint16_t* out, void* stream) {
+  clear_error();
+  const int rc = validate_int8_gemm("int8_gemm", a, a_scale, m, n, k, wq, ws, out);
+  if (rc != DSV4MOE_OK || m == 0) return rc;
+  return dsv4_launch_int8_gemm(a, a_scale, m, n, k, wq, ws, out, static_cast<hipStream_t>(stream));
+}
+
+int dsv4moe_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t n, int64_t k, const int8_t* wq,
+                        const uint16_t* ws, int8_t* q, float* scale, uint16_t* out, void* stream) {
+  clear_error();
+  int rc = validate_act_quant_int8("int8_linear", x, x_dtype, m, k, q, scale);
+  if (rc == DSV4MOE_OK) rc = validate_int8_gemm("int8_linear", q, scale, m, n, k, wq, ws, out);
+  if (rc != DSV4MOE_OK || m == 0) return rc;
+  rc = dsv4_launch_act_quant_int8(x, x_dtype, m, k, q, scale, static_cast<hipStream_t>(stream));
+  if (rc != DSV4MOE_OK) return rc;
+  return dsv4_launch_int8_gemm(q, scale, m, n, k, wq, ws, out, static_cast<hipStream_t>(stream));
+}
+
+// The checked parameters of a product by expert.
+static int grouped_params(const char* who, bool int8, const void* x, const float* x_scale, int64_t tokens,
+                          int32_t topk, int32_t per_slot, int64_t n, int64_t k, int32_t experts, const void* w,
+                          const uint16_t* ws, const int32_t* sorted_token_ids, int64_t capacity,
+                          const int32_t* expert_ids, const int32_t* num_tokens_post_padded, int32_t block_size,
+                          int32_t swiglu, float clamp_limit, const float* route_weights, uint16_t* out,
+                          dsv4::ProductParams* params) {
+  const int64_t limit = (int64_t)1 << 31;
+  const int itemsize = int8 ? 1 : 2;
+  DSV4_REQUIRE(tokens >= 0 && tokens < limit, "%s: tokens must be in [0, 2^31)", who);
+  DSV4_REQUIRE(topk > 0 && tokens * topk < limit, "%s: topk must be positive, tokens * topk below 2^31", who);
+  DSV4_REQUIRE(experts > 0, "%s: experts must be positive", who);
+  DSV4_REQUIRE(n > 0 && n < limit && n % (swiglu ? 32 : 16) == 0, "%s: n must be a positive multiple of %d, got %lld",
+               who, swiglu ? 32 : 16, (long long)n);
+  DSV4_REQUIRE(k > 0 && k < limit && k * itemsize % 16 == 0, "%s: rows of k must be a multiple of 16 bytes, got k = %lld",
+               who, (long long)k);
+  DSV4_REQUIRE(!int8 || k <= 65536, "%s: k must be <= 65536, got %lld", who, (long long)k);
+  const int64_t kbytes = k * itemsize, rows = per_slot ? tokens * topk : tokens;
+  DSV4_REQUIRE(n <= (limit - 1) / kbytes, "%s: an expert's weights must be below 2^31 bytes", who);
+  DSV4_REQUIRE(rows <= (limit - 1) / kbytes, "%s: x must be below 2^31 bytes", who);
+  DSV4_REQUIRE(block_size == 8 || block_size == 16 || block_size == 32 || block_size == 48 || block_size == 64,
+               "%s: block_size must be one of 8, 16, 32, 48, 64, got %d", who, block_size);
+  DSV4_REQUIRE(capacity > 0 && capacity < limit - block_size, "%s: bad capacity %lld", who, (long long)capacity);
+  const int64_t blocks = (capacity + block_size - 1) / block_size;
+  DSV4_REQUIRE((blocks + 8) * (n / 16) < limit, "%s: too many blocks and channels", who);
+  DSV4_REQUIRE(clamp_limit >= 0.0f, "%s: clamp_limit must be >= 0", who);
+  if (tokens == 0) return DSV4MOE_OK;
+  DSV4_REQUIRE(x && w && out && sorted_token_ids && expert_ids && num_tokens_post_padded && (!int8 || (x_scale && ws)),
+               "%s: null pointer", who);
+  DSV4_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(out, 16) && (!int8 || aligned(ws, 16)),
+               "%s: x, weights, their scales and out must be 16-byte aligned", who);
+  dsv4::ProductParams& p = *params;
+  p = dsv4::ProductParams{};
+  p.x = static_cast<const uint8_t*>(x);
+  p.rows = rows;
+  p.w = static_cast<const uint8_t*>(w);
+  p.n = (int)n;
+  p.kbytes = (int)kbytes;
+  p.kblocks = (int)((kbytes + dsv4::kBlockBytes - 1) / dsv4::kBlockBytes);
+  p.x_scale = x_scale;
+  p.w_scale = ws;
+  p.out = out;
+  p.out_n = (int)(swiglu ? n / 2 : n);
+  p.sorted_ids = sorted_token_ids;
+  p.expert_ids = expert_ids;
+  p.post_padded = num_tokens_post_padded;
+  p.capacity = (int)capacity;
+  p.blocks = (int)blocks;
+  p.block_size = block_size;
+  p.slots = (int)(tokens * topk);
+  p.per_row = per_slot ? 1 : topk;
+  p.experts = experts;
+  p.route_weights = route_weights;
+  p.clamp = clamp_limit;
+  return DSV4MOE_OK;
+}
+
+int dsv4moe_grouped_gemm(const uint16_t* x, int64_t tokens, int32_t topk, int32_t per_slot, int64_t n, int64_t k,
+                         int32_t experts, const uint16_t* w, const int32_t* sorted_token_ids, int64_t capacity,
+                         const int32_t* expert_ids, const int32_t* num_tokens_post_padded, int32_t block_size,
+                         int32_t swiglu, float clamp_limit, const float* route_weights, uint16_t* out, void* stream) {
+  clear_error();
+  dsv4::ProductParams p;
+  const int rc = grouped_params("grouped_gemm", false, x, nullptr, tokens, topk, per_slot, n, k, experts, w, nullptr,
+                                sorted_token_ids, capacity, expert_ids, num_tokens_post_padded, block_size, swiglu,
+                                clamp_limit, route_weights, out, &p);
+  if (rc != DSV4MOE_OK || tokens == 0) return rc;
+  return dsv4_launch_grouped(p, false, swiglu != 0, static_cast<hipStream_t>(stream));
+}
+
+int dsv4moe_grouped_int8_gemm(const int8_t* x, const float* x_scale, int64_t tokens, int32_t topk, int32_t per_slot,
+                              int64_t n, int64_t k, int32_t experts, const int8_t* w, const uint16_t* ws,
+                              const int32_t* sorted_token_ids, int64_t capacity, const int32_t* expert_ids,
+                              const int32_t* num_tokens_post_padded, int32_t block_size, int32_t swiglu,
+                              float clamp_limit, const float* route_weights, uint16_t* out, void* stream) {
+  clear_error();
+  dsv4::ProductParams p;
+  const int rc = grouped_params("grouped_int8_gemm", true, x, x_scale, tokens, topk, per_slot, n, k, experts, w, ws,
+                                sorted_token_ids, capacity, expert_ids, num_tokens_post_padded, block_size, swiglu,
+                                clamp_limit, route_weights, out, &p);
+  if (rc != DSV4MOE_OK || tokens == 0) return rc;
+  return dsv4_launch_grouped(p, true, swiglu != 0, static_cast<hipStream_t>(stream));
+}
+
+int dsv4moe_grouped_int8_linear(const void* x, int32_t x_dtype, int64_t tokens, int32_t topk, int32_t per_slot,
+                                int64_t n, int64_t k, int32_t experts, const int8_t* w, const uint16_t* ws,
+                                const int32_t* sorted_token_ids, int64_t capacity, const int32_t* expert_ids,
+                                const int32_t* num_tokens_post_padded, int32_t block_size, int32_t swiglu,
+                                float clamp_limit, const float* route_weights, int8_t* q, float* scale,
+                                uint16_t* out, void* stream) {
+  clear_error();
+  const char* who = "grouped_int8_linear";
+  dsv4::ProductParams p;
+  int rc = grouped_params(who, true, q, scale, tokens, topk, per_slot, n, k, experts, w, ws, sorted_token_ids, capacity,
+                          expert_ids, num_tokens_post_padded, block_size, swiglu, clamp_limit, route_weights, out, &p);
+  if (rc == DSV4MOE_OK) rc = validate_act_quant_int8(who, x, x_dtype, per_slot ? tokens * topk : tokens, k, q, scale);
+  if (rc != DSV4MOE_OK || tokens == 0) return rc;
+  rc = dsv4_launch_act_quant_int8(x, x_dtype, p.rows, k, q, scale, static_cast<hipStream_t>(stream));
+  if (rc != DSV4MOE_OK) return rc;
+  return dsv4_launch_grouped(p, true, swiglu != 0, static_cast<hipStream_t>(stream));
 }
 
 int32_t dsv4moe_block_fp8_split_k(int64_t m, int64_t n, int64_t k) { return dsv4_block_fp8_split_k(m, n, k); }

@@ -1,0 +1,357 @@
+// Products of activation rows with weight rows, out[i, n] = x[row(i), :] . W[n, :],
+// shared by the int8 linear (int8_linear.hip) and the linears grouped by expert
+// (grouped.hip).
+//
+// One operand layout serves both element types.  Rows are handled as bytes, in blocks
+// of 128 bytes of K (64 bf16 or 128 int8 values).  16 bytes are one lane's operand of
+// one MFMA in either type: 8 bf16 of v_mfma_f32_16x16x32_bf16 or 16 int8 of
+// v_mfma_i32_16x16x64_i8, lane group j = lane / 16 holding K bytes 16 j .. + 15 of a
+// 64-byte half block.  Weights are the MFMA's A operand (its rows are channels) and
+// activations its B operand, so a lane's four accumulators are four neighbouring
+// channels of one token.
+#pragma once
+
+#include "common.h"
+
+namespace dsv4 {
+
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
+constexpr int kTileXcds = 8;
+constexpr uint32_t kTileOob = 0x80000000u;  // beyond every buffer (each below 2^31 bytes): reads zeros
+constexpr int kTileRsrcFlags = 0x00020000;
+constexpr int kBlockBytes = 128;  // K bytes of a row per block
+
+struct ProductBf16 {
+  typedef f32x4 Acc;
+  static constexpr bool kInt8 = false;
+  __device__ static __forceinline__ Acc zero() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ static __forceinline__ Acc mfma(u32x4 w, u32x4 x, Acc c) {
+    return mfma_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), c);
+  }
+};
+struct ProductInt8 {
+  typedef i32x4 Acc;
+  static constexpr bool kInt8 = true;
+  __device__ static __forceinline__ Acc zero() { return i32x4{0, 0, 0, 0}; }
+  __device__ static __forceinline__ Acc mfma(u32x4 w, u32x4 x, Acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), c, 0, 0,
+                                                 0);
+  }
+};
+
+struct ProductParams {
+  const uint8_t* x;  // activation rows of `kbytes` bytes
+  int64_t rows;      // their number
+  const uint8_t* w;  // weight rows [n] of `kbytes` bytes, per expert
+  int n;
+  int kbytes;        // a multiple of 16
+  int kblocks;       // ceil(kbytes / 128)
+  int tiles_m, tiles_n;
+  const float* x_scale;     // int8: [rows]
+  const uint16_t* w_scale;  // int8: bf16 [experts][n]
+  uint16_t* out;
+  int out_n;         // channels of an output row: n, or n / 2 with SwiGLU
+  // grouped: the slots sorted by expert in padded blocks
+  const int32_t* sorted_ids;
+  const int32_t* expert_ids;
+  const int32_t* post_padded;
+  int capacity;      // of sorted_ids
+  int blocks;        // entries of expert_ids
+  int block_size;
+  int tile_blocks;   // blocks of one expert that a tile takes together
+  int slots;         // tokens * topk
+  int per_row;       // slots that one activation row serves (topk, or 1)
+  int experts;
+  const float* route_weights;  // [slots] or null
+  float clamp;
+};
+
+// The tile of grouped work item block `b`: a run of up to tile_blocks blocks of one
+// expert, taken by the run's first block (every tile_blocks-th block of its expert's);
+// nslots = 0 for a block that has no work of its own.  Called by whole wavefronts.
+struct GroupedTile {
+  int expert;
+  int first_slot;  // in sorted_ids
+  int nslots;
+};
+__device__ __forceinline__ GroupedTile grouped_tile(const ProductParams& p, int b) {
+  GroupedTile t{0, b * p.block_size, 0};
+  const int lane = threadIdx.x & 63;
+  const int active = min(p.blocks, *p.post_padded / p.block_size);  // none where the ids were out of range (-1)
+  if (b >= active) return t;
+  const int e = p.expert_ids[b];
+  if (e < 0 || e >= p.experts) return t;
+  if (p.tile_blocks > 1) {
+    // blocks of this expert before b: lane i looks at b - 1 - i, 64 at a time
+    int before = 0;
+    for (int at = b - 1; at >= 0; at -= 64) {
+      const int i = at - lane;
+      const uint64_t other = __ballot(i < 0 || p.expert_ids[max(i, 0)] != e);
+      if (other != 0) {
+        before += __builtin_ctzll(other);
+        break;
+      }
+      before += 64;
+    }
+    if (before % p.tile_blocks != 0) return t;
+    const int i = b + lane;
+    const uint64_t other = __ballot(lane >= p.tile_blocks || i >= active || p.expert_ids[min(i, active - 1)] != e);
+    t.nslots = __builtin_ctzll(other) * p.block_size;  // tile_blocks < 64: a bit is set
+  } else {
+    t.nslots = p.block_size;
+  }
+  t.expert = e;
+  return t;
+}
+
+// silu(min(g, L)) * clamp(u, -L, L), or without limits where L = 0
+__device__ __forceinline__ float swiglu_value(float g, float u, float limit) {
+  if (limit > 0.0f) {
+    g = fminf(g, limit);
+    u = fminf(fmaxf(u, -limit), limit);
+  }
+  return silu_f(g) * u;
+}
+
+// TOK rows x CH channels of WM x WN wavefronts, K in blocks of 128 bytes through a ring
+// of S stages in LDS.  buffer_load ... lds copies a stage (16-byte part q of row r at
+// q ^ swz128(r)); the copies of block kb + S - 1 are issued behind the barrier of block
+// kb, when every wavefront has read block kb - 1 out of the stage they refill, so S - 2
+// blocks are in flight while one is computed.  Wavefront (wm, wn) owns token columns
+// c * WM + wm (16 rows each; interleaved, so that a partly filled tile loads the
+// wavefronts alike) and strips wn * TN .. of the tile (16 channels each).  With SwiGLU a
+// wavefront's first TN / 2 strips are gate channels and the others the same up channels.
+template <class Op, int TOK, int CH, int WM, int WN, int S, bool GROUPED, bool SWIGLU>
+__global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParams p) {
+  constexpr int kWaves = WM * WN;
+  constexpr int TM = TOK / 16 / WM;
+  constexpr int TN = CH / 16 / WN;
+  constexpr int kStage = (TOK + CH) * kBlockBytes;
+  constexpr int kOutStrips = SWIGLU ? TN / 2 : TN;  // a wavefront's strips of output channels
+  static_assert(TM * 16 * WM == TOK && TN * 16 * WN == CH, "whole strips and columns per wavefront");
+  static_assert(!SWIGLU || TN % 2 == 0, "gate and up strips in one wavefront");
+  static_assert(CH / 8 % kWaves == 0, "every wavefront issues the same weight copies");
+  static_assert(TOK * kOutStrips * 16 * WN * 2 <= S * kStage, "the output tile fits the ring");
+  __shared__ __attribute__((aligned(16))) uint8_t ring[S * kStage];
+  __shared__ int row_id[TOK];  // the output row of each tile row, or -1
+  __shared__ float row_factor[TOK];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN;
+  const int wn = wave % WN;
+  const int n16 = lane & 15;
+  const int j = lane >> 4;
+
+  int tm, tn, expert = 0, first = 0, valid;
+  const uint8_t* xbase = p.x;
+  uint32_t xbytes;
+  if constexpr (GROUPED) {
+    // round robin over the XCDs by block; the channel tiles of a block on one XCD
+    const int at = blockIdx.x / kTileXcds;
+    tm = (at / p.tiles_n) * kTileXcds + blockIdx.x % kTileXcds;
+    tn = at % p.tiles_n;
+    const GroupedTile t = grouped_tile(p, tm);
+    valid = __builtin_amdgcn_readfirstlane(t.nslots);
+    if (valid == 0) return;
+    expert = __builtin_amdgcn_readfirstlane(t.expert);
+    first = t.first_slot;
+    xbytes = (uint32_t)(p.rows * p.kbytes);  // below 2^31 (host check)
+  } else {
+    const int items = p.tiles_m * p.tiles_n;
+    const int per_xcd = (items + kTileXcds - 1) / kTileXcds;
+    const int item = (blockIdx.x % kTileXcds) * per_xcd + blockIdx.x / kTileXcds;
+    if (item >= items) return;
+    tm = item / p.tiles_n;
+    tn = item % p.tiles_n;
+    const int64_t row0 = (int64_t)tm * TOK;
+    valid = (int)(p.rows - row0 < TOK ? p.rows - row0 : TOK);
+    xbase += row0 * p.kbytes;
+    xbytes = (uint32_t)valid * (uint32_t)p.kbytes;
+  }
+
+  // the tile's rows: activation row (for the copies) and output row
+  for (int r = threadIdx.x; r < TOK; r += 64 * kWaves) {
+    int id = -1;
+    if (r < valid) {
+      if constexpr (GROUPED) {
+        id = first + r < p.capacity ? p.sorted_ids[first + r] : -1;
+        if ((uint32_t)id >= (uint32_t)p.slots) id = -1;
+      } else {
+        id = r;
+      }
+    }
+    row_id[r] = id;
+    float f = 1.0f;
+    if (id >= 0) {
+      if constexpr (GROUPED) {
+        if (p.route_weights != nullptr) f = p.route_weights[id];
+      }
+    }
+    row_factor[r] = f;
+  }
+  __syncthreads();
+
+  const __amdgpu_buffer_rsrc_t x_rsrc =
+      __builtin_amdgcn_make_buffer_rsrc((void*)xbase, (short)0, (int)xbytes, kTileRsrcFlags);
+  const uint8_t* wbase = p.w + (int64_t)expert * p.n * p.kbytes;
+  const __amdgpu_buffer_rsrc_t w_rsrc =
+      __builtin_amdgcn_make_buffer_rsrc((void*)wbase, (short)0, (int)((int64_t)p.n * p.kbytes), kTileRsrcFlags);
+
+  // copy q of a stage fills its rows 8 q .. 8 q + 7 (tokens, then weights)
+  constexpr int kXCopies = (TOK / 8 + kWaves - 1) / kWaves;  // the last ones may repeat a row group
+  constexpr int kWCopies = CH / 8 / kWaves;
+  constexpr int kCopies = kXCopies + kWCopies;
+  uint32_t x_off[kXCopies], w_off[kWCopies];
+  uint32_t x_dst[kXCopies], w_dst[kWCopies];
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(&ring[0]));
+  uint32_t x_part[kXCopies], w_part[kWCopies];
+#pragma unroll
+  for (int i = 0; i < kXCopies; ++i) {
+    const int q = (wave + kWaves * i) % (TOK / 8);
+    const int row = q * 8 + (lane >> 3);
+    const int part = (lane & 7) ^ swz128(row);
+    const int id = row_id[row];
+    const uint32_t xr = GROUPED ? (uint32_t)id / (uint32_t)p.per_row : (uint32_t)id;
+    x_off[i] = id >= 0 ? xr * (uint32_t)p.kbytes + part * 16 : kTileOob;
+    x_part[i] = part * 16;
+    x_dst[i] = __builtin_amdgcn_readfirstlane(base + q * 1024);
+  }
+  const int half = p.n >> 1;
+#pragma unroll
+  for (int i = 0; i < kWCopies; ++i) {
+    const int q = wave + kWaves * i;
+    const int row = q * 8 + (lane >> 3);
+    const int part = (lane & 7) ^ swz128(row);
+    int ch;
+    bool in;
+    if constexpr (SWIGLU) {
+      const int strip = row >> 4, r = strip % TN;  // strip r of wavefront column strip / TN
+      ch = ((tn * WN + strip / TN) * kOutStrips + r % kOutStrips) * 16 + (row & 15);
+      in = ch < half;
+      ch += r < kOutStrips ? 0 : half;
+    } else {
+      ch = tn * CH + row;
+      in = ch < p.n;
+    }
+    w_off[i] = in ? (uint32_t)ch * (uint32_t)p.kbytes + part * 16 : kTileOob;
+    w_part[i] = part * 16;
+    w_dst[i] = __builtin_amdgcn_readfirstlane(base + TOK * kBlockBytes + q * 1024);
+  }
+  // Copies of block kb into stage `stage`.  Bytes past the end of K, and whole blocks past
+  // it (the ring runs on without a branch), are read out of range: zeros.
+  const int last = p.kblocks - 1;
+  const int tail = p.kbytes - last * kBlockBytes;  // bytes of the last block: 16 .. 128
+  auto copy = [&](int kb, int stage) {
+    const int soff = min(kb, last) * kBlockBytes;
+    const uint32_t limit = kb < last ? kBlockBytes : (kb == last ? tail : 0);
+    const uint32_t to = stage * kStage;
+#pragma unroll
+    for (int i = 0; i < kXCopies; ++i)
+      lds_copy16(x_rsrc, x_dst[i] + to, x_part[i] < limit ? x_off[i] : kTileOob, soff);
+#pragma unroll
+    for (int i = 0; i < kWCopies; ++i)
+      lds_copy16(w_rsrc, w_dst[i] + to, w_part[i] < limit ? w_off[i] : kTileOob, soff);
+  };
+
+  typename Op::Acc acc[TN][TM];
+#pragma unroll
+  for (int r = 0; r < TN; ++r)
+#pragma unroll
+    for (int c = 0; c < TM; ++c) acc[r][c] = Op::zero();
+
+  const int key = swz128(n16);
+  // the columns of this wavefront that hold rows
+  const int columns = (valid + 15) >> 4;
+  const int mine = columns > wm ? (columns - wm + WM - 1) / WM : 0;
+
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) copy(s, s);
+  int stage = 0;
+  for (int kb = 0; kb < p.kblocks; ++kb) {
+    lds_dma_wait_keep<(S - 2) * kCopies>();  // this wavefront's copies of block kb have landed
+    __syncthreads();                         // ... and everyone's; block kb - 1 has been read by all
+    copy(kb + S - 1, stage == 0 ? S - 1 : stage - 1);
+    const uint8_t* xs = &ring[stage * kStage];
+    const uint8_t* ws = xs + TOK * kBlockBytes;
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      u32x4 wf[TN];
+#pragma unroll
+      for (int r = 0; r < TN; ++r)
+        wf[r] = load16(ws + ((wn * TN + r) * 16 + n16) * kBlockBytes + (((4 * d + j) ^ key) * 16));
+#pragma unroll
+      for (int c = 0; c < TM; ++c) {
+        if (c >= mine) continue;
+        const u32x4 xf = load16(xs + ((c * WM + wm) * 16 + n16) * kBlockBytes + (((4 * d + j) ^ key) * 16));
+#pragma unroll
+        for (int r = 0; r < TN; ++r) acc[r][c] = Op::mfma(wf[r], xf, acc[r][c]);
+      }
+    }
+    stage = stage + 1 == S ? 0 : stage + 1;
+  }
+  lds_dma_wait_all();
+  __syncthreads();  // every wavefront has read its last fragments and its copies have landed
+
+  // Epilogue: the output tile through LDS, so that whole rows are stored.  16-byte part q
+  // of row r at q ^ (r mod parts).
+  constexpr int kParts = 2 * kOutStrips * WN;
+  constexpr int kRowBytes = 16 * kParts;
+  static_assert((kParts & (kParts - 1)) == 0, "parts of a row: a power of two");
+  float wscale[TN][4];
+  const int out_strip0 = (tn * WN + wn) * kOutStrips;
+  if constexpr (Op::kInt8) {
+#pragma unroll
+    for (int r = 0; r < TN; ++r) {
+      const int ch = (out_strip0 + (SWIGLU ? r % kOutStrips : r)) * 16 + 4 * j;
+      const int at = min(ch, p.out_n - 4) + (SWIGLU && r >= kOutStrips ? half : 0);
+      const u32x2 s = *reinterpret_cast<const u32x2*>(p.w_scale + (int64_t)expert * p.n + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wscale[r][e] = __uint_as_float((e & 1) ? s[e >> 1] & 0xFFFF0000u : s[e >> 1] << 16);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < TM; ++c) {
+    const int row = (c * WM + wm) * 16 + n16;
+    const int id = row_id[row];
+    const float factor = row_factor[row];
+    float xscale = 0.0f;
+    if constexpr (Op::kInt8) {
+      if (id >= 0) xscale = p.x_scale[GROUPED ? (int64_t)(id / p.per_row) : (int64_t)tm * TOK + id];
+    }
+    auto value = [&](int r, int e) {
+      if constexpr (Op::kInt8)
+        return (float)acc[r][c][e] * xscale * wscale[r][e];
+      else
+        return acc[r][c][e];
+    };
+#pragma unroll
+    for (int r = 0; r < kOutStrips; ++r) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (SWIGLU)
+          v[e] = swiglu_value(value(r, e), value(kOutStrips + r, e), p.clamp);
+        else
+          v[e] = value(r, e);
+        if constexpr (GROUPED) v[e] *= factor;
+      }
+      const int part = (2 * (wn * kOutStrips + r) + (j >> 1)) ^ (row & (kParts - 1));
+      *reinterpret_cast<u32x2*>(&ring[row * kRowBytes + part * 16 + (j & 1) * 8]) =
+          u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TOK * kParts; i += 64 * kWaves) {
+    const int row = i / kParts, q = i % kParts;
+    const int ch = tn * (kParts * 8) + q * 8;
+    const int id = row_id[row];
+    if (id < 0 || ch >= p.out_n) continue;
+    const int64_t dst = GROUPED ? (int64_t)id : (int64_t)tm * TOK + id;
+    *reinterpret_cast<u32x4*>(p.out + dst * p.out_n + ch) =
+        load16(&ring[row * kRowBytes + ((q ^ (row & (kParts - 1))) * 16)]);
+  }
+}
+
+}  // namespace dsv4

@@ -718,3 +718,129 @@ def shared_fp8_add_into(x: torch.Tensor, shared, *, clamp_limit: float, out: tor
     call("dsv4moe_shared_fp8_add", ptr(x), tokens, hidden, inter, ptr(shared.w13_q), ptr(shared.w13_s),
          ptr(shared.w2_q), ptr(shared.w2_s), float(clamp_limit), ptr(out), ptr(workspace), workspace.numel(),
          _lib.current_stream(dev))
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """``name(*args, stream)`` on ``device``'s current stream, with ``device``
+    current for the launch (it may differ from the caller's)."""
+
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _lib.current_stream(device))
+        return
+    with torch.cuda.device(device):
+        call(name, *args, _lib.current_stream(device))
+
+
+def _quant_dtype(x: torch.Tensor) -> int:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a tensor")
+    if x.ndim != 2:
+        raise ValueError("x must be [m, k]")
+    if x.dtype not in _X_DTYPE_CODES:
+        raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    return _X_DTYPE_CODES[x.dtype]
+
+
+def act_quant_int8_into(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """Per-token symmetric int8 quantisation (``dsv4moe_act_quant_int8``);
+    q int8 [m, k], scale fp32 [m]."""
+
+    code = _quant_dtype(x)
+    m, k = x.shape
+    dev = x.device
+    _check("x", x, dtype=x.dtype, device=dev)
+    _check("quantized_out", q, dtype=torch.int8, shape=(m, k), device=dev)
+    _check("scale_out", scale, dtype=torch.float32, shape=(m,), device=dev)
+    _launch(dev, "dsv4moe_act_quant_int8", ptr(x), code, m, k, ptr(q), ptr(scale))
+
+
+def int8_gemm_into(a: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+                   out: torch.Tensor) -> None:
+    """W8A8 int8 GEMM (``dsv4moe_int8_gemm``): a int8 [m, k] with fp32 a_scale
+    [m]; wq int8 [n, k] with bf16 ws [n]; out bf16 [m, n]."""
+
+    if a.ndim != 2 or wq.ndim != 2:
+        raise ValueError("activation must be [m, k] and weight [n, k]")
+    m, k = a.shape
+    n = wq.shape[0]
+    dev = a.device
+    _check("activation", a, dtype=torch.int8, device=dev)
+    _check("activation_scale", a_scale, dtype=torch.float32, shape=(m,), device=dev)
+    _check("weight", wq, dtype=torch.int8, shape=(n, k), device=dev)
+    _check("weight_scale", ws, dtype=torch.bfloat16, shape=(n,), device=dev)
+    _check("out", out, dtype=torch.bfloat16, shape=(m, n), device=dev)
+    _launch(dev, "dsv4moe_int8_gemm", ptr(a), ptr(a_scale), m, n, k, ptr(wq), ptr(ws), ptr(out))
+
+
+def int8_linear_into(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out: torch.Tensor, q: torch.Tensor,
+                     scale: torch.Tensor) -> None:
+    """``act_quant_int8_into`` and ``int8_gemm_into`` in one call
+    (``dsv4moe_int8_linear``); q int8 [m, k] and scale fp32 [m] are the call's
+    storage, their contents afterwards unspecified."""
+
+    code = _quant_dtype(x)
+    if wq.ndim != 2:
+        raise ValueError("weight must be [n, k]")
+    m, k = x.shape
+    n = wq.shape[0]
+    dev = x.device
+    _check("x", x, dtype=x.dtype, device=dev)
+    _check("weight", wq, dtype=torch.int8, shape=(n, k), device=dev)
+    _check("weight_scale", ws, dtype=torch.bfloat16, shape=(n,), device=dev)
+    _check("out", out, dtype=torch.bfloat16, shape=(m, n), device=dev)
+    _check("quantized", q, dtype=torch.int8, shape=(m, k), device=dev)
+    _check("scale", scale, dtype=torch.float32, shape=(m,), device=dev)
+    _launch(dev, "dsv4moe_int8_linear", ptr(x), code, m, n, k, ptr(wq), ptr(ws), ptr(q), ptr(scale), ptr(out))
+
+
+def grouped_gemm_into(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, tokens: int, topk: int,
+                      sorted_token_ids: torch.Tensor, expert_ids: torch.Tensor, num_tokens_post_padded: torch.Tensor,
+                      block_size: int, per_slot: bool = False, swiglu: bool = False, clamp_limit: float = 0.0,
+                      route_weights: torch.Tensor | None = None, x_scale: torch.Tensor | None = None,
+                      ws: torch.Tensor | None = None, quantized: torch.Tensor | None = None) -> None:
+    """Products by expert: x [tokens, k] (``per_slot``: [tokens * topk, k]),
+    w [experts, n, k], out bf16 [tokens * topk, n] (n / 2 with ``swiglu``),
+    the alignment of the routed ids at ``block_size``.
+
+    bf16 w: x bf16 (``dsv4moe_grouped_gemm``).  int8 w with bf16 scales ``ws``
+    [experts, n]: x int8 with fp32 ``x_scale`` [rows]
+    (``dsv4moe_grouped_int8_gemm``), or with ``quantized`` (int8, x's shape)
+    x bf16, fp16 or fp32, quantised into ``quantized`` and ``x_scale`` first
+    (``dsv4moe_grouped_int8_linear``)."""
+
+    if w.ndim != 3:
+        raise ValueError("weight must be [experts, n, k]")
+    experts, n, k = w.shape
+    slots = tokens * topk
+    rows = slots if per_slot else tokens
+    dev = x.device
+    int8 = w.dtype == torch.int8
+    if quantized is not None:
+        x_code = _quant_dtype(x)
+        _check("quantized", quantized, dtype=torch.int8, shape=(rows, k), device=dev)
+        _check("x", x, dtype=x.dtype, shape=(rows, k), device=dev)
+    else:
+        _check("x", x, dtype=torch.int8 if int8 else torch.bfloat16, shape=(rows, k), device=dev)
+    _check("weight", w, dtype=torch.int8 if int8 else torch.bfloat16, device=dev)
+    _check("out", out, dtype=torch.bfloat16, shape=(slots, n // 2 if swiglu else n), device=dev)
+    _check("sorted_token_ids", sorted_token_ids, dtype=torch.int32, device=dev)
+    capacity = sorted_token_ids.numel()
+    _check("expert_ids", expert_ids, dtype=torch.int32, shape=(-(-capacity // block_size),), device=dev)
+    _check("num_tokens_post_padded", num_tokens_post_padded, dtype=torch.int32, shape=(1,), device=dev)
+    if route_weights is not None:
+        _check("route_weights", route_weights, dtype=torch.float32, shape=(tokens, topk), device=dev)
+    if int8:
+        _check("activation_scale", x_scale, dtype=torch.float32, shape=(rows,), device=dev)
+        _check("weight_scale", ws, dtype=torch.bfloat16, shape=(experts, n), device=dev)
+    elif x_scale is not None or ws is not None or quantized is not None:
+        raise ValueError("only int8 weights take scales")
+    args = (tokens, topk, int(bool(per_slot)), n, k, experts, ptr(w))
+    rest = (ptr(sorted_token_ids), capacity, ptr(expert_ids), ptr(num_tokens_post_padded), block_size,
+            int(bool(swiglu)), float(clamp_limit), ptr(route_weights))
+    if quantized is not None:
+        _launch(dev, "dsv4moe_grouped_int8_linear", ptr(x), x_code, *args, ptr(ws), *rest, ptr(quantized),
+                ptr(x_scale), ptr(out))
+    elif int8:
+        _launch(dev, "dsv4moe_grouped_int8_gemm", ptr(x), ptr(x_scale), *args, ptr(ws), *rest, ptr(out))
+    else:
+        _launch(dev, "dsv4moe_grouped_gemm", ptr(x), *args, *rest, ptr(out))

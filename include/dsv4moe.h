@@ -561,6 +561,75 @@ int dsv4moe_dequant_mxfp4(const uint8_t* packed, const float* scale, int64_t row
 int dsv4moe_dequant_fp8_block(const void* w, int32_t w_dtype, const float* scale, int64_t rows, int64_t cols,
                               float* out, void* stream);
 
+/*
+ * W8A8 dense linear in 8-bit integers.  No counterpart in the reference, whose
+ * W8A8 linear is block-FP8 (runtime/dsv4_direct/fp8_linear.py): the integer
+ * form of the same call over the int8 weights of dsv4moe_w8a16_linear.
+ *
+ * dsv4moe_act_quant_int8: per-token symmetric quantiser.
+ *   x      [m, k] row-major, x_dtype DSV4MOE_DTYPE_BF16, _FP16 or _FP32
+ *   scale  fp32 [m] (out): s = max(amax, 1e-12) / 127, amax = the row's largest
+ *          magnitude; NaN for a row that holds a NaN or an infinity
+ *   q      int8 [m, k] (out): rint(x / s), half to even, in -127..127; 0 where s is NaN
+ * dsv4moe_int8_gemm:
+ *   out[m, n] = bf16( fp32(sum_k a[m, k] * wq[n, k]) * a_scale[m] * ws[n] ),
+ *   the sum exact in int32, the two products rounded in that order
+ *   a int8 [m, k]; a_scale fp32 [m]; wq int8 [n, k] row-major; ws bf16 [n]; out bf16 [m, n]
+ * dsv4moe_int8_linear: both from x.  q and scale are storage of the call: their
+ *   contents afterwards are unspecified.
+ * m >= 0, n % 16 == 0, k % 16 == 0, k <= 65536, n*k below 2^31; every pointer
+ * 16-byte aligned except scale and a_scale (4).
+ */
+int dsv4moe_act_quant_int8(const void* x, int32_t x_dtype, int64_t m, int64_t k, int8_t* q, float* scale,
+                           void* stream);
+int dsv4moe_int8_gemm(const int8_t* a, const float* a_scale, int64_t m, int64_t n, int64_t k, const int8_t* wq,
+                      const uint16_t* ws, uint16_t* out, void* stream);
+int dsv4moe_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t n, int64_t k, const int8_t* wq,
+                        const uint16_t* ws, int8_t* q, float* scale, uint16_t* out, void* stream);
+
+/*
+ * Linears grouped by expert over unfused weights [experts, n, k]: slot
+ * i = token * topk + j takes the weights of the expert it was aligned to,
+ *   y[i, :] = x[row(i), :] . W[e(i)]^T,  row(i) = per_slot ? i : i / topk,
+ *   out[i]  = bf16( r[i] * y[i] ), or with swiglu (n = 2 I, gate rows first)
+ *   out[i]  = bf16( r[i] * silu(min(g, L)) * clamp(u, -L, L) ), g = y[i, :I], u = y[i, I:]
+ * (no clamp when L = clamp_limit = 0; r = route_weights, 1 when NULL), fp32
+ * accumulation, int8 sums exact in int32 and scaled as in dsv4moe_int8_gemm.  The
+ * products of the experts' two linears, for experts kept in bf16 or int8
+ * (the reference keeps them in MXFP4: runtime/dsv4_direct/moe_runtime.py:1829-1856).
+ *   x        bf16 (grouped_gemm) or int8 (grouped_int8_gemm) [tokens or tokens*topk, k]
+ *   x_scale  fp32, one per row of x (dsv4moe_act_quant_int8)
+ *   w        bf16 or int8 [experts, n, k] row-major; ws bf16 [experts, n]
+ *   sorted_token_ids [capacity], expert_ids [ceil(capacity / block_size)],
+ *   num_tokens_post_padded: dsv4moe_align output, block_size in {8,16,32,48,64};
+ *            a sorted id outside [0, tokens*topk) is padding, a block whose expert id is
+ *            outside [0, experts) is skipped, and nothing is written when
+ *            num_tokens_post_padded is -1 (ids out of range)
+ *   route_weights fp32 [tokens * topk] or NULL
+ *   out      bf16 [tokens * topk, swiglu ? n / 2 : n]: the rows of the aligned slots
+ * dsv4moe_grouped_int8_linear: dsv4moe_act_quant_int8 of x (x_dtype) and
+ *   dsv4moe_grouped_int8_gemm; q (int8, x's shape) and scale (fp32, one per row) are
+ *   storage of the call.
+ * n % 16 == 0 (32 with swiglu); k % 8 == 0 (bf16) or 16 (int8, k <= 65536); n*k and
+ * x below 2^31 bytes each; pointers 16-byte aligned except x_scale, route_weights and
+ * the alignment (4).
+ */
+int dsv4moe_grouped_gemm(const uint16_t* x, int64_t tokens, int32_t topk, int32_t per_slot, int64_t n, int64_t k,
+                         int32_t experts, const uint16_t* w, const int32_t* sorted_token_ids, int64_t capacity,
+                         const int32_t* expert_ids, const int32_t* num_tokens_post_padded, int32_t block_size,
+                         int32_t swiglu, float clamp_limit, const float* route_weights, uint16_t* out, void* stream);
+int dsv4moe_grouped_int8_gemm(const int8_t* x, const float* x_scale, int64_t tokens, int32_t topk, int32_t per_slot,
+                              int64_t n, int64_t k, int32_t experts, const int8_t* w, const uint16_t* ws,
+                              const int32_t* sorted_token_ids, int64_t capacity, const int32_t* expert_ids,
+                              const int32_t* num_tokens_post_padded, int32_t block_size, int32_t swiglu,
+                              float clamp_limit, const float* route_weights, uint16_t* out, void* stream);
+int dsv4moe_grouped_int8_linear(const void* x, int32_t x_dtype, int64_t tokens, int32_t topk, int32_t per_slot,
+                                int64_t n, int64_t k, int32_t experts, const int8_t* w, const uint16_t* ws,
+                                const int32_t* sorted_token_ids, int64_t capacity, const int32_t* expert_ids,
+                                const int32_t* num_tokens_post_padded, int32_t block_size, int32_t swiglu,
+                                float clamp_limit, const float* route_weights, int8_t* q, float* scale,
+                                uint16_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
