@@ -2,7 +2,7 @@
 // activations quantised per token, weights int8 with one bf16 scale per output channel.
 // The products are summed exactly in int32 (K <= 65536: below 2^31), so the tiles, their
 // order and the K blocks do not show in the result.
-#include "product_tile.h"
+#include "product_gemm.h"
 #include "../../include/dsv4moe.h"
 
 namespace dsv4 {
@@ -123,6 +123,15 @@ static void launch_tile(ProductParams p, hipStream_t stream) {
                      stream, p);
 }
 
+template <int TOK, int CH, int WM, int WN>
+static void launch_gemm(ProductParams p, hipStream_t stream) {
+  p.tiles_m = (int)((p.rows + TOK - 1) / TOK);
+  p.tiles_n = (p.n + CH - 1) / CH;
+  const int items = p.tiles_m * p.tiles_n;
+  const dim3 grid((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds));
+  hipLaunchKernelGGL((product_gemm_kernel<ProductInt8, TOK, CH, WM, WN, false, false>), grid, dim3(512), 0, stream, p);
+}
+
 }  // namespace dsv4
 
 using namespace dsv4;
@@ -150,6 +159,7 @@ int dsv4_launch_int8_gemm(const int8_t* a, const float* a_scale, int64_t m, int6
   p.out = out;
   if (m <= 16) launch_tile<16, 64, 1, 4, 6>(p, stream);
   else if (m <= 64) launch_tile<64, 64, 2, 2, 4>(p, stream);
+  else if ((m + 255) / 256 * ((n + 255) / 256) >= 128) launch_gemm<256, 256, 4, 2>(p, stream);
   else launch_tile<128, 128, 2, 2, 3>(p, stream);
   DSV4_CHECK_LAUNCH("product_tile_kernel");
   return DSV4MOE_OK;

@@ -114,6 +114,142 @@ __device__ __forceinline__ float swiglu_value(float g, float u, float limit) {
   return silu_f(g) * u;
 }
 
+// The rows of a tile, by the whole workgroup.
+template <int TOK>
+struct TileRows {
+  int id[TOK];                    // output row, or -1
+  float factor[TOK];              // its route weight
+  int used[(TOK + 63) / 64];      // rows up to the last that has one, per 64
+
+  // `count` rows from sorted slot `first` on (grouped) or the first `count` (dense)
+  template <bool GROUPED>
+  __device__ __forceinline__ void fill(const ProductParams& p, int first, int count) {
+    for (int r = threadIdx.x; r < TOK; r += blockDim.x) {
+      int i = -1;
+      float f = 1.0f;
+      if (r < count) {
+        if constexpr (GROUPED) {
+          if (first + r < p.capacity) i = p.sorted_ids[first + r];
+          if ((uint32_t)i >= (uint32_t)p.slots) i = -1;
+          if (i >= 0 && p.route_weights != nullptr) f = p.route_weights[i];
+        } else {
+          i = r;
+        }
+      }
+      id[r] = i;
+      factor[r] = f;
+      const uint64_t have = __ballot(i >= 0);
+      if ((r & 63) == 0) used[r >> 6] = have ? (r & ~63) + 64 - __builtin_clzll(have) : 0;
+    }
+  }
+  // behind a barrier: rows up to the last that has an output
+  __device__ __forceinline__ int rows() const {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < (TOK + 63) / 64; ++i) n = max(n, used[i]);
+    return __builtin_amdgcn_readfirstlane(n);
+  }
+};
+
+// Byte offset in the activations of output row `id`, or out of range for -1.
+template <bool GROUPED>
+__device__ __forceinline__ uint32_t x_row_offset(const ProductParams& p, int id) {
+  const uint32_t row = GROUPED ? (uint32_t)id / (uint32_t)p.per_row : (uint32_t)id;
+  return id >= 0 ? row * (uint32_t)p.kbytes : kTileOob;
+}
+
+// Byte offset in the expert's weights of row `row` of channel tile tn (WN wavefront columns
+// of TN strips), or out of range past the last channel.
+template <int CH, int TN, int WN, bool SWIGLU>
+__device__ __forceinline__ uint32_t w_row_offset(const ProductParams& p, int tn, int row) {
+  int ch;
+  bool in;
+  if constexpr (SWIGLU) {
+    const int strip = row >> 4, r = strip % TN;  // strip r of wavefront column strip / TN
+    const int half = p.n >> 1;
+    ch = ((tn * WN + strip / TN) * (TN / 2) + r % (TN / 2)) * 16 + (row & 15);
+    in = ch < half;
+    ch += r < TN / 2 ? 0 : half;
+  } else {
+    ch = tn * CH + row;
+    in = ch < p.n;
+  }
+  return in ? (uint32_t)ch * (uint32_t)p.kbytes : kTileOob;
+}
+
+// The workgroup's finished tile to the output, through `lds` (TOK rows of all its output
+// channels) so that whole rows are stored: 16-byte part q of row r is kept at
+// q ^ (r mod parts).  Every wavefront has read its last fragments from `lds`.
+template <class Op, int TOK, int TM, int TN, int WM, int WN, bool GROUPED, bool SWIGLU>
+__device__ __forceinline__ void store_tile(const ProductParams& p, const typename Op::Acc (&acc)[TN][TM],
+                                           uint8_t* lds, const TileRows<TOK>& rows, int tm, int tn, int expert) {
+  constexpr int kWaves = WM * WN;
+  constexpr int kOutStrips = SWIGLU ? TN / 2 : TN;  // a wavefront's strips of output channels
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN;
+  const int wn = wave % WN;
+  const int n16 = lane & 15;
+  const int j = lane >> 4;
+  const int half = p.n >> 1;
+  constexpr int kParts = 2 * kOutStrips * WN;
+  constexpr int kRowBytes = 16 * kParts;
+  static_assert((kParts & (kParts - 1)) == 0, "parts of a row: a power of two");
+  float wscale[TN][4];
+  const int out_strip0 = (tn * WN + wn) * kOutStrips;
+  if constexpr (Op::kInt8) {
+#pragma unroll
+    for (int r = 0; r < TN; ++r) {
+      const int ch = (out_strip0 + (SWIGLU ? r % kOutStrips : r)) * 16 + 4 * j;
+      const int at = min(ch, p.out_n - 4) + (SWIGLU && r >= kOutStrips ? half : 0);
+      const u32x2 s = *reinterpret_cast<const u32x2*>(p.w_scale + (int64_t)expert * p.n + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wscale[r][e] = __uint_as_float((e & 1) ? s[e >> 1] & 0xFFFF0000u : s[e >> 1] << 16);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < TM; ++c) {
+    const int row = (c * WM + wm) * 16 + n16;
+    const int id = rows.id[row];
+    const float factor = rows.factor[row];
+    float xscale = 0.0f;
+    if constexpr (Op::kInt8) {
+      if (id >= 0) xscale = p.x_scale[GROUPED ? (int64_t)(id / p.per_row) : (int64_t)tm * TOK + id];
+    }
+    auto value = [&](int r, int e) {
+      if constexpr (Op::kInt8)
+        return (float)acc[r][c][e] * xscale * wscale[r][e];
+      else
+        return acc[r][c][e];
+    };
+#pragma unroll
+    for (int r = 0; r < kOutStrips; ++r) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (SWIGLU)
+          v[e] = swiglu_value(value(r, e), value(kOutStrips + r, e), p.clamp);
+        else
+          v[e] = value(r, e);
+        if constexpr (GROUPED) v[e] *= factor;
+      }
+      const int part = (2 * (wn * kOutStrips + r) + (j >> 1)) ^ (row & (kParts - 1));
+      *reinterpret_cast<u32x2*>(&lds[row * kRowBytes + part * 16 + (j & 1) * 8]) =
+          u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TOK * kParts; i += 64 * kWaves) {
+    const int row = i / kParts, q = i % kParts;
+    const int ch = tn * (kParts * 8) + q * 8;
+    const int id = rows.id[row];
+    if (id < 0 || ch >= p.out_n) continue;
+    const int64_t dst = GROUPED ? (int64_t)id : (int64_t)tm * TOK + id;
+    *reinterpret_cast<u32x4*>(p.out + dst * p.out_n + ch) =
+        load16(&lds[row * kRowBytes + ((q ^ (row & (kParts - 1))) * 16)]);
+  }
+}
+
 // TOK rows x CH channels of WM x WN wavefronts, K in blocks of 128 bytes through a ring
 // of S stages in LDS.  buffer_load ... lds copies a stage (16-byte part q of row r at
 // q ^ swz128(r)); the copies of block kb + S - 1 are issued behind the barrier of block
@@ -134,8 +270,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   static_assert(CH / 8 % kWaves == 0, "every wavefront issues the same weight copies");
   static_assert(TOK * kOutStrips * 16 * WN * 2 <= S * kStage, "the output tile fits the ring");
   __shared__ __attribute__((aligned(16))) uint8_t ring[S * kStage];
-  __shared__ int row_id[TOK];  // the output row of each tile row, or -1
-  __shared__ float row_factor[TOK];
+  __shared__ TileRows<TOK> rows;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -171,27 +306,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
     xbytes = (uint32_t)valid * (uint32_t)p.kbytes;
   }
 
-  // the tile's rows: activation row (for the copies) and output row
-  for (int r = threadIdx.x; r < TOK; r += 64 * kWaves) {
-    int id = -1;
-    if (r < valid) {
-      if constexpr (GROUPED) {
-        id = first + r < p.capacity ? p.sorted_ids[first + r] : -1;
-        if ((uint32_t)id >= (uint32_t)p.slots) id = -1;
-      } else {
-        id = r;
-      }
-    }
-    row_id[r] = id;
-    float f = 1.0f;
-    if (id >= 0) {
-      if constexpr (GROUPED) {
-        if (p.route_weights != nullptr) f = p.route_weights[id];
-      }
-    }
-    row_factor[r] = f;
-  }
+  rows.template fill<GROUPED>(p, first, valid);
   __syncthreads();
+  valid = rows.rows();
 
   const __amdgpu_buffer_rsrc_t x_rsrc =
       __builtin_amdgcn_make_buffer_rsrc((void*)xbase, (short)0, (int)xbytes, kTileRsrcFlags);
@@ -212,30 +329,16 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
     const int q = (wave + kWaves * i) % (TOK / 8);
     const int row = q * 8 + (lane >> 3);
     const int part = (lane & 7) ^ swz128(row);
-    const int id = row_id[row];
-    const uint32_t xr = GROUPED ? (uint32_t)id / (uint32_t)p.per_row : (uint32_t)id;
-    x_off[i] = id >= 0 ? xr * (uint32_t)p.kbytes + part * 16 : kTileOob;
+    x_off[i] = x_row_offset<GROUPED>(p, rows.id[row]) + part * 16;
     x_part[i] = part * 16;
     x_dst[i] = __builtin_amdgcn_readfirstlane(base + q * 1024);
   }
-  const int half = p.n >> 1;
 #pragma unroll
   for (int i = 0; i < kWCopies; ++i) {
     const int q = wave + kWaves * i;
     const int row = q * 8 + (lane >> 3);
     const int part = (lane & 7) ^ swz128(row);
-    int ch;
-    bool in;
-    if constexpr (SWIGLU) {
-      const int strip = row >> 4, r = strip % TN;  // strip r of wavefront column strip / TN
-      ch = ((tn * WN + strip / TN) * kOutStrips + r % kOutStrips) * 16 + (row & 15);
-      in = ch < half;
-      ch += r < kOutStrips ? 0 : half;
-    } else {
-      ch = tn * CH + row;
-      in = ch < p.n;
-    }
-    w_off[i] = in ? (uint32_t)ch * (uint32_t)p.kbytes + part * 16 : kTileOob;
+    w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, row) + part * 16;
     w_part[i] = part * 16;
     w_dst[i] = __builtin_amdgcn_readfirstlane(base + TOK * kBlockBytes + q * 1024);
   }
@@ -294,64 +397,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   lds_dma_wait_all();
   __syncthreads();  // every wavefront has read its last fragments and its copies have landed
 
-  // Epilogue: the output tile through LDS, so that whole rows are stored.  16-byte part q
-  // of row r at q ^ (r mod parts).
-  constexpr int kParts = 2 * kOutStrips * WN;
-  constexpr int kRowBytes = 16 * kParts;
-  static_assert((kParts & (kParts - 1)) == 0, "parts of a row: a power of two");
-  float wscale[TN][4];
-  const int out_strip0 = (tn * WN + wn) * kOutStrips;
-  if constexpr (Op::kInt8) {
-#pragma unroll
-    for (int r = 0; r < TN; ++r) {
-      const int ch = (out_strip0 + (SWIGLU ? r % kOutStrips : r)) * 16 + 4 * j;
-      const int at = min(ch, p.out_n - 4) + (SWIGLU && r >= kOutStrips ? half : 0);
-      const u32x2 s = *reinterpret_cast<const u32x2*>(p.w_scale + (int64_t)expert * p.n + at);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) wscale[r][e] = __uint_as_float((e & 1) ? s[e >> 1] & 0xFFFF0000u : s[e >> 1] << 16);
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < TM; ++c) {
-    const int row = (c * WM + wm) * 16 + n16;
-    const int id = row_id[row];
-    const float factor = row_factor[row];
-    float xscale = 0.0f;
-    if constexpr (Op::kInt8) {
-      if (id >= 0) xscale = p.x_scale[GROUPED ? (int64_t)(id / p.per_row) : (int64_t)tm * TOK + id];
-    }
-    auto value = [&](int r, int e) {
-      if constexpr (Op::kInt8)
-        return (float)acc[r][c][e] * xscale * wscale[r][e];
-      else
-        return acc[r][c][e];
-    };
-#pragma unroll
-    for (int r = 0; r < kOutStrips; ++r) {
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (SWIGLU)
-          v[e] = swiglu_value(value(r, e), value(kOutStrips + r, e), p.clamp);
-        else
-          v[e] = value(r, e);
-        if constexpr (GROUPED) v[e] *= factor;
-      }
-      const int part = (2 * (wn * kOutStrips + r) + (j >> 1)) ^ (row & (kParts - 1));
-      *reinterpret_cast<u32x2*>(&ring[row * kRowBytes + part * 16 + (j & 1) * 8]) =
-          u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < TOK * kParts; i += 64 * kWaves) {
-    const int row = i / kParts, q = i % kParts;
-    const int ch = tn * (kParts * 8) + q * 8;
-    const int id = row_id[row];
-    if (id < 0 || ch >= p.out_n) continue;
-    const int64_t dst = GROUPED ? (int64_t)id : (int64_t)tm * TOK + id;
-    *reinterpret_cast<u32x4*>(p.out + dst * p.out_n + ch) =
-        load16(&ring[row * kRowBytes + ((q ^ (row & (kParts - 1))) * 16)]);
-  }
+  store_tile<Op, TOK, TM, TN, WM, WN, GROUPED, SWIGLU>(p, acc, ring, rows, tm, tn, expert);
 }
 
 }  // namespace dsv4
