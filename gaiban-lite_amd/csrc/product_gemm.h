@@ -92,11 +92,11 @@ struct NoTileList {};
 // columns c * WM + wm and strips wn * TN .. as in product_tile_kernel.  Half the strips'
 // fragments are held, a strip's registers being refilled behind its MFMAs with the strip
 // half a block later; the rows' fragments of the next block are read during the second
-// half.  So no MFMA waits for the reads of eight wavefronts at once, and the barrier stands
-// in the middle of a block, when the rest of the block is in registers: block kb + 1 has
-// landed by then, and the copies of block kb + 2 refill block kb's stage.  The LDS holds
-// one block ahead, less than a first read takes, so four blocks ahead one dword of each
-// 128-byte line is touched (copied to a dump), which brings the line into L2.
+// half.  So no MFMA waits for the reads of eight wavefronts at once, and what has been
+// read of a block (its rows and first strips when it begins, the other strips in its
+// middle) makes room for the copies of block kb + 2 at once: each lands one and a half
+// blocks later.  The two barriers of a block stand behind a strip's MFMAs, so that the
+// reads before them have landed.
 //
 // Grouped: the workgroups stay and walk the items (tile, channel tile) of their XCD's share
 // in that order, so one XCD's L2 serves an expert's rows to all its channel tiles.  Columns
@@ -110,10 +110,8 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   constexpr int kStage = (TOK + CH) * kBlockBytes;
   static_assert(kWaves == 8 && TM * 16 * WM == TOK && TN * 16 * WN == CH && TN % 2 == 0, "eight wavefronts");
   static_assert(TM <= 2 * H, "two columns' fragments per strip of the second half");
-  static_assert(TOK / 8 % kWaves == 0 && CH / 8 % kWaves == 0, "every wavefront issues the same copies");
-  static_assert(TOK % 64 == 0 && CH % 64 == 0 && TOK / 64 + CH / 64 <= kWaves, "one touch per wavefront");
+  static_assert(TOK / 8 % kWaves == 0 && CH / 16 % kWaves == 0, "every wavefront issues the same copies");
   __shared__ __attribute__((aligned(16))) uint8_t ring[2 * kStage];
-  __shared__ __attribute__((aligned(16))) uint32_t dump[64];
   __shared__ TileRows<TOK> rows;
   __shared__ std::conditional_t<GROUPED, TileList, NoTileList> list;
 
@@ -127,13 +125,20 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   const int last = p.kblocks - 1;
   const uint32_t tail = p.kbytes - last * kBlockBytes;  // bytes of the last block
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(&ring[0]));
-  const uint32_t dump_lds = __builtin_amdgcn_readfirstlane(lds_addr(&dump[0]));
   constexpr int kXCopies = TOK / 8 / kWaves;
   constexpr int kWCopies = CH / 8 / kWaves;
   constexpr int kCopies = kXCopies + kWCopies;
-  // the 16-byte part of a row that this lane copies: the same in all its copies, which are
-  // rows 8 q .. with q = wave + 8 i
+  constexpr int kEarly = kXCopies + kWCopies / 2;  // copies of the part of a block that is read first
+  // the 16-byte part of a row that this lane copies: the same in all its copies, groups of
+  // eight rows that are odd or even with the wavefront
   const uint32_t part = ((lane & 7) ^ (lane >> 3) ^ (wave & 1)) * 16;
+
+  // the group of eight weight rows that copy i fills: first those of the wavefront columns'
+  // strips below H, then the others
+  auto w_group = [&](int i) {
+    const int l = wave + kWaves * (i % (kWCopies / 2));
+    return l / (2 * H) * 2 * TN + l % (2 * H) + (i < kWCopies / 2 ? 0 : 2 * H);
+  };
 
   auto tile = [&](int tm, int tn, int expert, int first, int count, const uint8_t* xbase, uint32_t xbytes) {
     rows.template fill<GROUPED>(p, first, count);
@@ -149,7 +154,7 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
       x_off[i] = x_row_offset<GROUPED>(p, rows.id[(wave + kWaves * i) * 8 + (lane >> 3)]) + part;
 #pragma unroll
     for (int i = 0; i < kWCopies; ++i)
-      w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, (wave + kWaves * i) * 8 + (lane >> 3)) + part;
+      w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, w_group(i) * 8 + (lane >> 3)) + part;
     // One copy of block kb into stage `u`; past the end of K: zeros.
     auto copy = [&](int kb, int u, int i) {
       const uint32_t limit = kb < last ? kBlockBytes : (kb == last ? tail : 0);
@@ -157,22 +162,9 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
       if (i < kXCopies)
         lds_copy16(x_rsrc, base + u * kStage + (wave + kWaves * i) * 1024, part < limit ? x_off[i] : kTileOob, soff);
       else
-        lds_copy16(w_rsrc, base + u * kStage + TOK * kBlockBytes + (wave + kWaves * (i - kXCopies)) * 1024,
+        lds_copy16(w_rsrc, base + u * kStage + TOK * kBlockBytes + w_group(i - kXCopies) * 1024,
                    part < limit ? w_off[i - kXCopies] : kTileOob, soff);
     };
-    // Touched lines: wavefront w < CH / 64 weight rows 64 w .. + 63, the next ones activation
-    // rows.  Tiles that run together on an XCD share them: of a dense call's weights each
-    // touches a quarter (the kGemmGroup token tiles beside it the rest), of the activations
-    // an eighth.
-    uint32_t touch_off = kTileOob;
-    if (wave < CH / 64) {
-      if (GROUPED || CH / 64 < 4 || (tm & 3) == wave) touch_off = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, wave * 64 + lane);
-    } else if (wave < CH / 64 + TOK / 64) {
-      if (lane / 8 == (tn & 7)) touch_off = x_row_offset<GROUPED>(p, rows.id[(wave - CH / 64) * 64 + lane]);
-    }
-    const __amdgpu_buffer_rsrc_t touch_rsrc = wave < CH / 64 ? w_rsrc : x_rsrc;
-    auto touch = [&](int kb) { lds_copy4(touch_rsrc, dump_lds, touch_off, min(kb, last) * kBlockBytes); };
-
     typename Op::Acc acc[TN][TM];
 #pragma unroll
     for (int r = 0; r < TN; ++r)
@@ -193,9 +185,7 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
     for (int i = 0; i < kCopies; ++i) copy(0, 0, i);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) copy(1, 1, i);
-    touch(2);
-    touch(3);
-    lds_dma_wait_keep<kCopies + 2>();
+    lds_dma_wait_keep<2 * kCopies - kEarly>();
     __syncthreads();
 
     auto loop = [&](auto cols_c) __attribute__((always_inline)) {
@@ -205,23 +195,27 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
         constexpr int u = decltype(u_c)::value;
 #pragma unroll
         for (int r = 0; r < TN; ++r) {
-          if (r == H) {
-            lds_dma_wait_keep<1>();  // this wavefront's copies of block kb + 1 have landed (the touch may be in flight)
-            __syncthreads();         // ... and everyone's; the rest of block kb is in registers
-          }
+          // copies of block kb + 2 into what has been read of block kb: spread over the strips
+          // behind the barrier
+          const int first = r < H ? 0 : kEarly, count = r < H ? kEarly : kCopies - kEarly;
+          const int slots = (H - 1) * 2 * COLS, at = (r % H - 1) * 2 * COLS;
 #pragma unroll
           for (int m = 0; m < 2 * COLS; ++m) {
             const int d = m / COLS, c = m % COLS;
             acc[r][c] = Op::mfma(wf[r % H].d[d], cur[c].d[d], acc[r][c]);
             __builtin_amdgcn_sched_barrier(0);
-            if (r >= H) {
-              constexpr int kSlots = H * 2 * COLS;
-              const int slot = (r - H) * 2 * COLS + m;
+            if (r % H > 0) {
 #pragma unroll
-              for (int i = 0; i < kCopies; ++i)
-                if (i * kSlots / kCopies == slot) copy(kb + 2, u, i);
-              if (slot == kSlots - 1) touch(kb + 4);
+              for (int i = 0; i < count; ++i)
+                if (i * slots / count == at + m) copy(kb + 2, u, first + i);
             }
+          }
+          if (r % H == 0) {
+            // Strip 0: the later part of block kb has landed, and every wavefront has its
+            // rows and first strips of block kb in registers.  Strip H: the early part of
+            // block kb + 1 has landed, the rest of block kb is in registers.
+            lds_dma_wait_keep<kCopies>();
+            __syncthreads();
           }
           wf[r % H] = r < H ? read_strip(u, r + H) : read_strip(u ^ 1, r - H);
           if (r >= H) {
