@@ -127,8 +127,8 @@ template <int TOK, int CH, int WM, int WN>
 static void launch_gemm(ProductParams p, hipStream_t stream) {
   p.tiles_m = (int)((p.rows + TOK - 1) / TOK);
   p.tiles_n = (p.n + CH - 1) / CH;
-  const int items = p.tiles_m * p.tiles_n;
-  const dim3 grid((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds));
+  const int64_t items = ((int64_t)p.tiles_m * p.tiles_n + kTileXcds - 1) / kTileXcds * kTileXcds;
+  const dim3 grid((unsigned)(items < kGemmCus ? items : kGemmCus));
   hipLaunchKernelGGL((product_gemm_kernel<ProductInt8, TOK, CH, WM, WN, false, false>), grid, dim3(512), 0, stream, p);
 }
 
@@ -159,7 +159,8 @@ int dsv4_launch_int8_gemm(const int8_t* a, const float* a_scale, int64_t m, int6
   p.out = out;
   if (m <= 16) launch_tile<16, 64, 1, 4, 6>(p, stream);
   else if (m <= 64) launch_tile<64, 64, 2, 2, 4>(p, stream);
-  else if ((m + 255) / 256 * ((n + 255) / 256) >= 128) launch_gemm<256, 256, 4, 2>(p, stream);
+  else if ((m + 255) / 256 * ((n + 255) / 256) >= 192) launch_gemm<256, 256, 4, 2>(p, stream);
+  else if ((m + 255) / 256 * ((n + 127) / 128) >= 192) launch_gemm<256, 128, 4, 2>(p, stream);
   else launch_tile<128, 128, 2, 2, 3>(p, stream);
   DSV4_CHECK_LAUNCH("product_tile_kernel");
   return DSV4MOE_OK;

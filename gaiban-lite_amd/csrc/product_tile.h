@@ -111,7 +111,7 @@ __device__ __forceinline__ float swiglu_value(float g, float u, float limit) {
     g = fminf(g, limit);
     u = fminf(fmaxf(u, -limit), limit);
   }
-  return silu_f(g) * u;
+  return silu_rcp(g) * u;
 }
 
 // The rows of a tile, by the whole workgroup.
