@@ -140,7 +140,6 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   const int wn = wave % WN;
   const int n16 = lane & 15;
   const int j = lane >> 4;
-  const int key = swz128(n16);
   const int last = p.kblocks - 1;
   const int steps = (p.kblocks + 1) & ~1;  // an odd number of blocks: one more of zeros
   const uint32_t tail = p.kbytes - last * kBlockBytes;  // bytes of the last block
@@ -149,9 +148,10 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   constexpr int kWCopies = CH / 8 / kWaves;
   constexpr int kCopies = kXCopies + kWCopies;
   constexpr int kEarly = kXCopies + kWCopies / 2;  // copies of the part of a block that is read first
-  // the 16-byte part of a row that this lane copies: the same in all its copies, groups of
-  // eight rows that are odd or even with the wavefront
-  const uint32_t part = ((lane & 7) ^ (lane >> 3) ^ (wave & 1)) * 16;
+  // the row of each group of eight and its 16-byte part that this lane copies: the same in
+  // all its copies
+  const int lane_row = lane >> 3;
+  const uint32_t part = lds_part(lane_row, lane & 7) * 16;
   // the group of eight weight rows that copy i fills: first those of the wavefront columns'
   // strips below H, then the others
   auto w_group = [&](int i) {
@@ -222,17 +222,17 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
       xbytes = t.count > 0 ? (uint32_t)(p.rows * p.kbytes) : 0;  // below 2^31 (host check)
 #pragma unroll
       for (int i = 0; i < kXCopies; ++i)
-        x_off[i] = x_row_offset<true>(p, t.count > 0 ? rows[slot].id[(wave + kWaves * i) * 8 + (lane >> 3)] : -1) + part;
+        x_off[i] = x_row_offset<true>(p, t.count > 0 ? rows[slot].id[(wave + kWaves * i) * 8 + lane_row] : -1) + part;
     } else {
       xbase += (int64_t)t.tm * TOK * p.kbytes;
       xbytes = (uint32_t)t.count * (uint32_t)p.kbytes;
-      x_off[0] = (uint32_t)(wave * 8 + (lane >> 3)) * (uint32_t)p.kbytes + part;
+      x_off[0] = (uint32_t)(wave * 8 + lane_row) * (uint32_t)p.kbytes + part;
     }
     x_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)xbase, (short)0, (int)xbytes, kTileRsrcFlags);
     const uint8_t* wbase = p.w + (int64_t)t.expert * p.n * p.kbytes;
     const int wbytes = t.count > 0 ? (int)((int64_t)p.n * p.kbytes) : 0;
     w_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)wbase, (short)0, wbytes, kTileRsrcFlags);
-    w_off = (uint32_t)(t.tn * (SWIGLU ? CH / 2 : CH) + w_group(0) * 8 + (lane >> 3)) * (uint32_t)p.kbytes + part;
+    w_off = (uint32_t)(t.tn * (SWIGLU ? CH / 2 : CH) + w_group(0) * 8 + lane_row) * (uint32_t)p.kbytes + part;
   };
   // Rows from the first weight row of a wavefront's copies to that of copy i.  Eight groups of
   // rows (the wavefronts' copies) are four strips.
@@ -267,8 +267,8 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   };
   // fragment addresses: strips, columns and stages are constants beside two lane addresses
   // each (part 4 + j lies at the other half of part j's row, 64 bytes off)
-  uint32_t x_lds = base + (wm * 16 + n16) * kBlockBytes + ((j ^ key) * 16);
-  uint32_t w_lds = base + 2 * kXStage + (wn * TN * 16 + n16) * kBlockBytes + ((j ^ key) * 16);
+  uint32_t x_lds = base + (wm * 16 + n16) * kBlockBytes + lds_part(n16, j) * 16;
+  uint32_t w_lds = base + 2 * kXStage + (wn * TN * 16 + n16) * kBlockBytes + lds_part(n16, j) * 16;
   uint32_t x_lds4 = x_lds ^ 64, w_lds4 = w_lds ^ 64;
   opaque(x_lds), opaque(x_lds4), opaque(w_lds), opaque(w_lds4);
   auto read_strip = [&](int u, int r) __attribute__((always_inline)) {

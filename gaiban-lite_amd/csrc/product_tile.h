@@ -40,6 +40,14 @@ struct ProductInt8 {
   }
 };
 
+// Where 16-byte part `part` of a row of a block lies in its 128 bytes of LDS.  The LDS serves
+// a ds_read_b128 in sets of 16 lanes (0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of each half of
+// a wavefront: measured by moving one lane at a time onto another's banks); with part j of
+// row r at j ^ (r & 7), lanes (row r, part j = lane / 16) of a set fall into all sixteen slots
+// of the 256 bytes of banks (SQ_LDS_BANK_CONFLICT 0; swz128's order, made for other reads, has
+// four conflicts a read here).
+__device__ __forceinline__ int lds_part(int row, int part) { return part ^ (row & 7); }
+
 struct ProductParams {
   const uint8_t* x;  // activation rows of `kbytes` bytes
   int64_t rows;      // their number
@@ -251,8 +259,7 @@ __device__ __forceinline__ void store_tile(const ProductParams& p, const typenam
 }
 
 // TOK rows x CH channels of WM x WN wavefronts, K in blocks of 128 bytes through a ring
-// of S stages in LDS.  buffer_load ... lds copies a stage (16-byte part q of row r at
-// q ^ swz128(r)); the copies of block kb + S - 1 are issued behind the barrier of block
+// of S stages in LDS.  buffer_load ... lds copies a stage (16-byte parts as lds_part says); the copies of block kb + S - 1 are issued behind the barrier of block
 // kb, when every wavefront has read block kb - 1 out of the stage they refill, so S - 2
 // blocks are in flight while one is computed.  Wavefront (wm, wn) owns token columns
 // c * WM + wm (16 rows each; interleaved, so that a partly filled tile loads the
@@ -328,7 +335,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   for (int i = 0; i < kXCopies; ++i) {
     const int q = (wave + kWaves * i) % (TOK / 8);
     const int row = q * 8 + (lane >> 3);
-    const int part = (lane & 7) ^ swz128(row);
+    const int part = lds_part(row, lane & 7);
     x_off[i] = x_row_offset<GROUPED>(p, rows.id[row]) + part * 16;
     x_part[i] = part * 16;
     x_dst[i] = __builtin_amdgcn_readfirstlane(base + q * 1024);
@@ -337,7 +344,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   for (int i = 0; i < kWCopies; ++i) {
     const int q = wave + kWaves * i;
     const int row = q * 8 + (lane >> 3);
-    const int part = (lane & 7) ^ swz128(row);
+    const int part = lds_part(row, lane & 7);
     w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, row) + part * 16;
     w_part[i] = part * 16;
     w_dst[i] = __builtin_amdgcn_readfirstlane(base + TOK * kBlockBytes + q * 1024);
@@ -364,7 +371,6 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
 #pragma unroll
     for (int c = 0; c < TM; ++c) acc[r][c] = Op::zero();
 
-  const int key = swz128(n16);
   // the columns of this wavefront that hold rows
   const int columns = (valid + 15) >> 4;
   const int mine = columns > wm ? (columns - wm + WM - 1) / WM : 0;
@@ -383,11 +389,11 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
       u32x4 wf[TN];
 #pragma unroll
       for (int r = 0; r < TN; ++r)
-        wf[r] = load16(ws + ((wn * TN + r) * 16 + n16) * kBlockBytes + (((4 * d + j) ^ key) * 16));
+        wf[r] = load16(ws + ((wn * TN + r) * 16 + n16) * kBlockBytes + lds_part(n16, 4 * d + j) * 16);
 #pragma unroll
       for (int c = 0; c < TM; ++c) {
         if (c >= mine) continue;
-        const u32x4 xf = load16(xs + ((c * WM + wm) * 16 + n16) * kBlockBytes + (((4 * d + j) ^ key) * 16));
+        const u32x4 xf = load16(xs + ((c * WM + wm) * 16 + n16) * kBlockBytes + lds_part(n16, 4 * d + j) * 16);
 #pragma unroll
         for (int r = 0; r < TN; ++r) acc[r][c] = Op::mfma(wf[r], xf, acc[r][c]);
       }
