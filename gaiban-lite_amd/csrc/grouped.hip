@@ -10,7 +10,7 @@ static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
   p.tile_blocks = TOK / p.block_size;
   p.tiles_m = p.blocks;
   p.tiles_n = (p.n + CH - 1) / CH;
-  const dim3 grid((unsigned)((p.blocks + kTileXcds - 1) / kTileXcds * kTileXcds * p.tiles_n));
+  const dim3 grid((unsigned)(p.blocks * p.tiles_n));
   hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, S, true, SWIGLU>), grid, dim3(64 * WM * WN), 0, stream, p);
 }
 

@@ -290,10 +290,10 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   const uint8_t* xbase = p.x;
   uint32_t xbytes;
   if constexpr (GROUPED) {
-    // round robin over the XCDs by block; the channel tiles of a block on one XCD
-    const int at = blockIdx.x / kTileXcds;
-    tm = (at / p.tiles_n) * kTileXcds + blockIdx.x % kTileXcds;
-    tn = at % p.tiles_n;
+    // neighbouring workgroups, which run on different XCDs, take neighbouring channel tiles:
+    // few blocks still use every XCD
+    tm = blockIdx.x / p.tiles_n;
+    tn = blockIdx.x % p.tiles_n;
     const GroupedTile t = grouped_tile(p, tm);
     valid = __builtin_amdgcn_readfirstlane(t.nslots);
     if (valid == 0) return;
@@ -313,10 +313,6 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
     xbytes = (uint32_t)valid * (uint32_t)p.kbytes;
   }
 
-  rows.template fill<GROUPED>(p, first, valid);
-  __syncthreads();
-  valid = rows.rows();
-
   const __amdgpu_buffer_rsrc_t x_rsrc =
       __builtin_amdgcn_make_buffer_rsrc((void*)xbase, (short)0, (int)xbytes, kTileRsrcFlags);
   const uint8_t* wbase = p.w + (int64_t)expert * p.n * p.kbytes;
@@ -330,40 +326,42 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   uint32_t x_off[kXCopies], w_off[kWCopies];
   uint32_t x_dst[kXCopies], w_dst[kWCopies];
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(&ring[0]));
-  uint32_t x_part[kXCopies], w_part[kWCopies];
-#pragma unroll
-  for (int i = 0; i < kXCopies; ++i) {
-    const int q = (wave + kWaves * i) % (TOK / 8);
-    const int row = q * 8 + (lane >> 3);
-    const int part = lds_part(row, lane & 7);
-    x_off[i] = x_row_offset<GROUPED>(p, rows.id[row]) + part * 16;
-    x_part[i] = part * 16;
-    x_dst[i] = __builtin_amdgcn_readfirstlane(base + q * 1024);
-  }
+  // Every copy of a lane is of the same 16-byte part.  Bytes past the end of K, and whole
+  // blocks past it (the ring runs on without a branch), are read out of range: zeros.
+  const uint32_t part = lds_part(lane >> 3, lane & 7) * 16;
+  const int last = p.kblocks - 1;
+  const uint32_t tail = p.kbytes - last * kBlockBytes;  // bytes of the last block: 16 .. 128
+  auto limit = [&](int kb) { return kb < last ? kBlockBytes : (kb == last ? tail : 0); };
 #pragma unroll
   for (int i = 0; i < kWCopies; ++i) {
     const int q = wave + kWaves * i;
-    const int row = q * 8 + (lane >> 3);
-    const int part = lds_part(row, lane & 7);
-    w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, row) + part * 16;
-    w_part[i] = part * 16;
+    w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, q * 8 + (lane >> 3)) + part;
     w_dst[i] = __builtin_amdgcn_readfirstlane(base + TOK * kBlockBytes + q * 1024);
   }
-  // Copies of block kb into stage `stage`.  Bytes past the end of K, and whole blocks past
-  // it (the ring runs on without a branch), are read out of range: zeros.
-  const int last = p.kblocks - 1;
-  const int tail = p.kbytes - last * kBlockBytes;  // bytes of the last block: 16 .. 128
-  auto copy = [&](int kb, int stage) {
-    const int soff = min(kb, last) * kBlockBytes;
-    const uint32_t limit = kb < last ? kBlockBytes : (kb == last ? tail : 0);
-    const uint32_t to = stage * kStage;
-#pragma unroll
-    for (int i = 0; i < kXCopies; ++i)
-      lds_copy16(x_rsrc, x_dst[i] + to, x_part[i] < limit ? x_off[i] : kTileOob, soff);
+  auto copy_w = [&](int kb, int stage) {
 #pragma unroll
     for (int i = 0; i < kWCopies; ++i)
-      lds_copy16(w_rsrc, w_dst[i] + to, w_part[i] < limit ? w_off[i] : kTileOob, soff);
+      lds_copy16(w_rsrc, w_dst[i] + stage * kStage, part < limit(kb) ? w_off[i] : kTileOob, min(kb, last) * kBlockBytes);
   };
+  auto copy_x = [&](int kb, int stage) {
+#pragma unroll
+    for (int i = 0; i < kXCopies; ++i)
+      lds_copy16(x_rsrc, x_dst[i] + stage * kStage, part < limit(kb) ? x_off[i] : kTileOob, min(kb, last) * kBlockBytes);
+  };
+  // the first weights do not wait for the rows' ids
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) copy_w(s, s);
+  rows.template fill<GROUPED>(p, first, valid);
+  __syncthreads();
+  valid = rows.rows();
+#pragma unroll
+  for (int i = 0; i < kXCopies; ++i) {
+    const int q = (wave + kWaves * i) % (TOK / 8);
+    x_off[i] = x_row_offset<GROUPED>(p, rows.id[q * 8 + (lane >> 3)]) + part;
+    x_dst[i] = __builtin_amdgcn_readfirstlane(base + q * 1024);
+  }
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) copy_x(s, s);
 
   typename Op::Acc acc[TN][TM];
 #pragma unroll
@@ -375,13 +373,16 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   const int columns = (valid + 15) >> 4;
   const int mine = columns > wm ? (columns - wm + WM - 1) / WM : 0;
 
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s) copy(s, s);
   int stage = 0;
   for (int kb = 0; kb < p.kblocks; ++kb) {
-    lds_dma_wait_keep<(S - 2) * kCopies>();  // this wavefront's copies of block kb have landed
-    __syncthreads();                         // ... and everyone's; block kb - 1 has been read by all
-    copy(kb + S - 1, stage == 0 ? S - 1 : stage - 1);
+    // this wavefront's copies of block kb have landed (the first S - 1 blocks' weights were
+    // copied ahead of their rows)
+    if (kb < S - 2) lds_dma_wait_keep<(S - 2) * kXCopies>();
+    else lds_dma_wait_keep<(S - 2) * kCopies>();
+    __syncthreads();  // ... and everyone's; block kb - 1 has been read by all
+    const int refill = stage == 0 ? S - 1 : stage - 1;
+    copy_x(kb + S - 1, refill);
+    copy_w(kb + S - 1, refill);
     const uint8_t* xs = &ring[stage * kStage];
     const uint8_t* ws = xs + TOK * kBlockBytes;
 #pragma unroll
