@@ -69,6 +69,8 @@ static void prof_release() {
 int dsv4_launch_act_quant_int8(const void*, int32_t, int64_t, int64_t, int8_t*, float*, hipStream_t);
 int dsv4_launch_int8_gemm(const int8_t*, const float*, int64_t, int64_t, int64_t, const int8_t*, const uint16_t*,
                           uint16_t*, hipStream_t);
+int dsv4_launch_int8_linear(const void*, int32_t, int64_t, int64_t, int64_t, const int8_t*, const uint16_t*, int8_t*,
+                            float*, uint16_t*, hipStream_t);
 int dsv4_launch_grouped(const dsv4::ProductParams&, bool, bool, hipStream_t);
 int dsv4_launch_route_topk(const float*, const float*, int64_t, int32_t, int32_t, int32_t, float,
                            int32_t*, float*, float*, int32_t*, float*, hipStream_t);
@@ -961,9 +963,7 @@ int dsv4moe_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t n, in
   int rc = validate_act_quant_int8("int8_linear", x, x_dtype, m, k, q, scale);
   if (rc == DSV4MOE_OK) rc = validate_int8_gemm("int8_linear", q, scale, m, n, k, wq, ws, out);
   if (rc != DSV4MOE_OK || m == 0) return rc;
-  rc = dsv4_launch_act_quant_int8(x, x_dtype, m, k, q, scale, static_cast<hipStream_t>(stream));
-  if (rc != DSV4MOE_OK) return rc;
-  return dsv4_launch_int8_gemm(q, scale, m, n, k, wq, ws, out, static_cast<hipStream_t>(stream));
+  return dsv4_launch_int8_linear(x, x_dtype, m, n, k, wq, ws, q, scale, out, static_cast<hipStream_t>(stream));
 }
 
 // The checked parameters of a product by expert.

@@ -5,13 +5,14 @@
 
 namespace dsv4 {
 
-template <class Op, int TOK, int CH, int WM, int WN, int S, bool SWIGLU>
+template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool SWIGLU>
 static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
   p.tile_blocks = TOK / p.block_size;
   p.tiles_m = p.blocks;
   p.tiles_n = (p.n + CH - 1) / CH;
   const dim3 grid((unsigned)(p.blocks * p.tiles_n));
-  hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, S, true, SWIGLU>), grid, dim3(64 * WM * WN), 0, stream, p);
+  hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU>), grid, dim3(64 * WM * WN * WK), 0, stream,
+                     p);
 }
 
 template <class Op, int TOK, int CH, int WM, int WN, bool SWIGLU>
@@ -27,8 +28,9 @@ template <class Op, bool SWIGLU>
 static void launch_grouped(const ProductParams& p, hipStream_t stream) {
   const int per_expert = p.slots / p.experts;
   if (per_expert >= 64) return launch_grouped_gemm<Op, 256, 256, 4, 2, SWIGLU>(p, stream);
-  if (p.block_size <= 16) launch_grouped_tile<Op, 16, 64, 1, 2, 6, SWIGLU>(p, stream);
-  else launch_grouped_tile<Op, 64, 128, 1, 4, 3, SWIGLU>(p, stream);
+  if (p.block_size <= 16) launch_grouped_tile<Op, 16, 32, 1, 1, 4, 2, SWIGLU>(p, stream);
+  else if (p.block_size <= 32) launch_grouped_tile<Op, 32, 128, 1, 4, 2, 3, SWIGLU>(p, stream);
+  else launch_grouped_tile<Op, 64, 128, 2, 4, 1, 3, SWIGLU>(p, stream);
 }
 
 }  // namespace dsv4

@@ -113,13 +113,169 @@ static void launch_quant(const void* x, int64_t m, int k, int8_t* q, float* scal
                        q, scale);
 }
 
-template <int TOK, int CH, int WM, int WN, int S>
+// ------------------------------------------------------------ few tokens
+// Up to 16 tokens in one launch: every workgroup quantises all of them into LDS (while its
+// first weights are under way) and then streams strips of 16 channels.  The K of a strip is
+// dealt out in slices of 256 bytes to eight wavefronts; a wavefront copies its own slices, 16
+// rows x 256 bytes at a time, into kFewStages stages of its own, so that nothing but the end
+// of a strip needs a barrier: there the eight partial sums (exact, int32) are added.  A lane
+// whose token does not exist reads another's codes, for a column that nothing stores.
+struct FewParams {
+  const void* x;
+  int m, n, k;
+  const uint8_t* w;
+  const uint16_t* ws;
+  uint16_t* out;
+};
+constexpr int kFewWaves = 8;
+constexpr int kFewStages = 3;
+constexpr int kFewSlice = 256;                      // K bytes of a wavefront per stage
+constexpr int kFewRound = kFewWaves * kFewSlice;    // K bytes of a workgroup per stage
+constexpr int kFewRing = kFewWaves * kFewStages * 16 * kFewSlice;
+constexpr int kFewCodes = 44 * 1024;                // all tokens' codes
+
+static int64_t few_code_bytes(int64_t m, int64_t k) { return m * ((k + kFewRound - 1) / kFewRound * kFewRound); }
+
+__device__ __forceinline__ void lds_wait_all() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#endif
+}
+
+template <int X>
+__global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t lds[kFewRing];
+  __shared__ __attribute__((aligned(256))) uint8_t codes[kFewCodes];  // [m][rounds * kFewRound]
+  __shared__ i32x4 sums[2][kFewWaves][64];
+  __shared__ uint32_t amax_of[16][kFewWaves];
+  __shared__ float scale_of[16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n16 = lane & 15;
+  const int j = lane >> 4;
+  const int strips = p.n >> 4;
+  const int rounds = (p.k + kFewRound - 1) / kFewRound;
+  const int code_row = rounds * kFewRound;
+
+  // this wavefront's copies: 4 rows x 256 bytes each, part q of row r at q ^ r
+  const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_addr(lds + wave * kFewStages * 16 * kFewSlice));
+  const int copy_row = lane >> 4;
+  const __amdgpu_buffer_rsrc_t w_rsrc =
+      __builtin_amdgcn_make_buffer_rsrc((void*)p.w, (short)0, (int)((int64_t)p.n * p.k), kTileRsrcFlags);
+  const int mine = strips > (int)blockIdx.x ? (strips - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+  const int steps = mine * rounds;  // over this workgroup's strips
+  auto copy = [&](int step, int stage) {
+    const int strip = blockIdx.x + step / rounds * gridDim.x;
+    const int k0 = step % rounds * kFewRound + wave * kFewSlice;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 4 + copy_row;
+      const int at = k0 + lds_part<kFewSlice>(row, lane & 15) * 16;
+      const uint32_t off = step < steps && at < p.k ? (uint32_t)((strip * 16 + row) * p.k + at) : kTileOob;
+      lds_copy16(w_rsrc, ring + stage * 16 * kFewSlice + i * 1024, off, 0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kFewStages - 1; ++s) copy(s, s);
+
+  // quantise: each row by all threads, 8 values at a time
+  const int chunks = p.k / 8;
+  for (int r = 0; r < p.m; ++r) {
+    uint32_t amax = 0;
+    for (int c = threadIdx.x; c < chunks; c += 512) {
+      float f[8];
+      load8_as_float<X>(p.x, (int64_t)r * p.k + c * 8, f);
+      amax = max_magnitude(amax, f);
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, off, 64));
+    if (lane == 0) amax_of[r][wave] = amax;
+  }
+  __syncthreads();
+  for (int r = 0; r < p.m; ++r) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) amax = max(amax, amax_of[r][w]);
+    const float s = int8_row_scale(amax);
+    if (threadIdx.x == 0) scale_of[r] = s;
+    for (int c = threadIdx.x; c < code_row / 8; c += 512) {
+      u32x2 q = {0, 0};
+      if (c < chunks) {
+        float f[8];
+        load8_as_float<X>(p.x, (int64_t)r * p.k + c * 8, f);
+        q = int8_codes(f, s);
+      }
+      // 16-byte parts of each 256 bytes in the order of the weights' rows
+      const int at = (c >> 5) * kFewSlice + lds_part<kFewSlice>(r, c >> 1 & 15) * 16 + (c & 1) * 8;
+      *reinterpret_cast<u32x2*>(codes + r * code_row + at) = q;
+    }
+  }
+  __syncthreads();
+
+  const int token = n16 % p.m;
+  const uint8_t* my_codes = codes + token * code_row + wave * kFewSlice;
+  i32x4 acc = {0, 0, 0, 0};
+  int stage = 0, turn = 0;
+  for (int step = 0; step < steps; ++step) {
+    lds_dma_wait_keep<(kFewStages - 2) * 4>();
+    const uint8_t* ws = lds + (wave * kFewStages + stage) * 16 * kFewSlice;
+    const uint8_t* xs = my_codes + step % rounds * kFewRound;
+    u32x4 wf[4], xf[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      wf[d] = load16(ws + n16 * kFewSlice + lds_part<kFewSlice>(n16, 4 * d + j) * 16);
+      xf[d] = load16(xs + lds_part<kFewSlice>(token, 4 * d + j) * 16);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) acc = ProductInt8::mfma(wf[d], xf[d], acc);
+    // the fragments are in registers before their stage is filled again
+    lds_wait_all();
+    const int refill = stage == 0 ? kFewStages - 1 : stage - 1;
+    copy(step + kFewStages - 1, refill);
+    stage = stage + 1 == kFewStages ? 0 : stage + 1;
+    if ((step + 1) % rounds != 0) continue;
+    // the end of a strip (two sets of sums in turn: one barrier)
+    sums[turn][wave][lane] = acc;
+    acc = i32x4{0, 0, 0, 0};
+    __syncthreads();
+    if (wave == (step / rounds) % kFewWaves) {
+      const int strip = blockIdx.x + step / rounds * gridDim.x;
+      i32x4 total = sums[turn][0][lane];
+#pragma unroll
+      for (int w = 1; w < kFewWaves; ++w) total += sums[turn][w][lane];
+      if (n16 < p.m) {
+        const float xs16 = scale_of[n16];
+        const u32x2 s = *reinterpret_cast<const u32x2*>(p.ws + strip * 16 + 4 * j);
+        const float w4[4] = {__uint_as_float(s[0] << 16), __uint_as_float(s[0] & 0xFFFF0000u),
+                             __uint_as_float(s[1] << 16), __uint_as_float(s[1] & 0xFFFF0000u)};
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)total[e] * xs16 * w4[e];
+        *reinterpret_cast<u32x2*>(p.out + (int64_t)n16 * p.n + strip * 16 + 4 * j) =
+            u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      }
+    }
+    turn ^= 1;
+  }
+  lds_dma_wait_all();
+}
+
+template <int X>
+static int launch_few(const FewParams& p, hipStream_t stream) {
+  const int strips = p.n / 16;
+  hipLaunchKernelGGL((int8_few_kernel<X>), dim3((unsigned)(strips < kGemmCus ? strips : kGemmCus)), dim3(512), 0,
+                     stream, p);
+  DSV4_CHECK_LAUNCH("int8_few_kernel");
+  return DSV4MOE_OK;
+}
+
+template <int TOK, int CH, int WM, int WN, int WK, int S>
 static void launch_tile(ProductParams p, hipStream_t stream) {
   p.tiles_m = (int)((p.rows + TOK - 1) / TOK);
   p.tiles_n = (p.n + CH - 1) / CH;
   const int items = p.tiles_m * p.tiles_n;
   const dim3 grid((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds));
-  hipLaunchKernelGGL((product_tile_kernel<ProductInt8, TOK, CH, WM, WN, S, false, false>), grid, dim3(64 * WM * WN), 0,
+  hipLaunchKernelGGL((product_tile_kernel<ProductInt8, TOK, CH, WM, WN, WK, S, false, false>), grid, dim3(64 * WM * WN * WK), 0,
                      stream, p);
 }
 
@@ -130,6 +286,34 @@ static void launch_gemm(ProductParams p, hipStream_t stream) {
   const int64_t items = ((int64_t)p.tiles_m * p.tiles_n + kTileXcds - 1) / kTileXcds * kTileXcds;
   const dim3 grid((unsigned)(items < kGemmCus ? items : kGemmCus));
   hipLaunchKernelGGL((product_gemm_kernel<ProductInt8, TOK, CH, WM, WN, false, false>), grid, dim3(512), 0, stream, p);
+}
+
+// The tile with the least time by a model: a start, then its workgroups' share of tiles per
+// CU times the K blocks, each block's time measured on a full card (us, 128 bytes of K):
+// 32 x 64 0.175, 64 x 64 0.25, 128 x 128 0.47, 256 x 128 0.85, 256 x 256 1.62 (it takes 54
+// against 59, 66, 128 and 179 us of a CU per 256 x 256 outputs and 32 blocks; the smaller
+// ones are for grids that would leave CUs idle).  Measured with the quantiser, N=K=4096: M=64
+// 13.0 / 16.5 / 19.2 / 27.7 / 43.3 us, M=300 22.8 / 19.5 / 20.6 / 29.5 / 44.9, M=2000
+// 99.6 / 74.9 / 44.1 / 40.5 / 52.3.
+static void launch_product(const ProductParams& p, hipStream_t stream) {
+  struct Tile {
+    int tok, ch;
+    double start, block;
+    void (*launch)(ProductParams, hipStream_t);
+  };
+  static const Tile tiles[] = {
+      {32, 64, 3.4, 0.175, launch_tile<32, 64, 1, 2, 2, 3>}, {64, 64, 4.0, 0.25, launch_tile<64, 64, 2, 4, 1, 3>},
+      {128, 128, 2.0, 0.47, launch_gemm<128, 128, 4, 2>},    {256, 128, 3.0, 0.85, launch_gemm<256, 128, 4, 2>},
+      {256, 256, 3.0, 1.62, launch_gemm<256, 256, 4, 2>},
+  };
+  const Tile* best = nullptr;
+  double least = 0.0;
+  for (const Tile& t : tiles) {
+    const int64_t items = (p.rows + t.tok - 1) / t.tok * ((p.n + t.ch - 1) / t.ch);
+    const double time = t.start + (double)((items + kGemmCus - 1) / kGemmCus) * p.kblocks * t.block;
+    if (best == nullptr || time < least) best = &t, least = time;
+  }
+  best->launch(p, stream);
 }
 
 }  // namespace dsv4
@@ -157,11 +341,21 @@ int dsv4_launch_int8_gemm(const int8_t* a, const float* a_scale, int64_t m, int6
   p.x_scale = a_scale;
   p.w_scale = ws;
   p.out = out;
-  if (m <= 16) launch_tile<16, 64, 1, 4, 6>(p, stream);
-  else if (m <= 64) launch_tile<64, 64, 2, 2, 4>(p, stream);
-  else if ((m + 255) / 256 * ((n + 255) / 256) >= 192) launch_gemm<256, 256, 4, 2>(p, stream);
-  else if ((m + 255) / 256 * ((n + 127) / 128) >= 192) launch_gemm<256, 128, 4, 2>(p, stream);
-  else launch_tile<128, 128, 2, 2, 3>(p, stream);
+  launch_product(p, stream);
   DSV4_CHECK_LAUNCH("product_tile_kernel");
   return DSV4MOE_OK;
+}
+
+// One launch, or the quantiser and the product.
+int dsv4_launch_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t n, int64_t k, const int8_t* wq,
+                            const uint16_t* ws, int8_t* q, float* scale, uint16_t* out, hipStream_t stream) {
+  if (m <= 16 && few_code_bytes(m, k) <= kFewCodes) {
+    const FewParams p{x, (int)m, (int)n, (int)k, reinterpret_cast<const uint8_t*>(wq), ws, out};
+    if (x_dtype == DSV4MOE_DTYPE_BF16) return launch_few<DSV4MOE_DTYPE_BF16>(p, stream);
+    if (x_dtype == DSV4MOE_DTYPE_FP16) return launch_few<DSV4MOE_DTYPE_FP16>(p, stream);
+    return launch_few<DSV4MOE_DTYPE_FP32>(p, stream);
+  }
+  const int rc = dsv4_launch_act_quant_int8(x, x_dtype, m, k, q, scale, stream);
+  if (rc != DSV4MOE_OK) return rc;
+  return dsv4_launch_int8_gemm(q, scale, m, n, k, wq, ws, out, stream);
 }

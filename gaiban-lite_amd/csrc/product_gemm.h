@@ -151,12 +151,23 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   // the row of each group of eight and its 16-byte part that this lane copies: the same in
   // all its copies
   const int lane_row = lane >> 3;
-  const uint32_t part = lds_part(lane_row, lane & 7) * 16;
+  const uint32_t part = lds_part<128>(lane_row, lane & 7) * 16;
   // the group of eight weight rows that copy i fills: first those of the wavefront columns'
   // strips below H, then the others
   auto w_group = [&](int i) {
     const int l = wave + kWaves * (i % (kWCopies / 2));
     return l / (2 * H) * 2 * TN + l % (2 * H) + (i < kWCopies / 2 ? 0 : 2 * H);
+  };
+
+  // the first channel of a group of eight weight rows, from the tile's first
+  auto w_row = [&](int group) {
+    const int strip = group >> 1;
+    if constexpr (SWIGLU) {
+      const int r = strip % TN;
+      return (strip / TN * (TN / 2) + r % (TN / 2)) * 16 + (group & 1) * 8 + (r < TN / 2 ? 0 : p.n >> 1);
+    } else {
+      return group * 8;
+    }
   };
 
   // ---- the items of this workgroup
@@ -232,18 +243,7 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
     const uint8_t* wbase = p.w + (int64_t)t.expert * p.n * p.kbytes;
     const int wbytes = t.count > 0 ? (int)((int64_t)p.n * p.kbytes) : 0;
     w_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)wbase, (short)0, wbytes, kTileRsrcFlags);
-    w_off = (uint32_t)(t.tn * (SWIGLU ? CH / 2 : CH) + w_group(0) * 8 + lane_row) * (uint32_t)p.kbytes + part;
-  };
-  // Rows from the first weight row of a wavefront's copies to that of copy i.  Eight groups of
-  // rows (the wavefronts' copies) are four strips.
-  auto w_rows = [&](int i) {
-    const int strip = (w_group(i) - w_group(0)) / 2;  // whole strips: groups differ by even numbers
-    if constexpr (SWIGLU) {
-      const int r = strip % TN;
-      return (strip / TN * (TN / 2) + r % (TN / 2)) * 16 + (r < TN / 2 ? 0 : p.n >> 1);
-    } else {
-      return strip * 16;
-    }
+    w_off = (uint32_t)(t.tn * (SWIGLU ? CH / 2 : CH) + w_row(w_group(0)) + lane_row) * (uint32_t)p.kbytes + part;
   };
   // One copy of block kb into stage `u`; past the end of K: zeros.
   auto copy = [&](int kb, int u, int i) __attribute__((always_inline)) {
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
       if constexpr (!GROUPED) off += kWaves * 8 * i * (uint32_t)p.kbytes;
       lds_copy16(x_rsrc, base + u * kXStage + (wave + kWaves * i) * 1024, off, soff);
     } else {
-      off += (uint32_t)w_rows(i - kXCopies) * (uint32_t)p.kbytes;
+      off += (uint32_t)(w_row(w_group(i - kXCopies)) - w_row(w_group(0))) * (uint32_t)p.kbytes;
       lds_copy16(w_rsrc, base + 2 * kXStage + u * kWStage + w_group(i - kXCopies) * 1024, off, soff);
     }
   };
@@ -267,8 +267,8 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   };
   // fragment addresses: strips, columns and stages are constants beside two lane addresses
   // each (part 4 + j lies at the other half of part j's row, 64 bytes off)
-  uint32_t x_lds = base + (wm * 16 + n16) * kBlockBytes + lds_part(n16, j) * 16;
-  uint32_t w_lds = base + 2 * kXStage + (wn * TN * 16 + n16) * kBlockBytes + lds_part(n16, j) * 16;
+  uint32_t x_lds = base + (wm * 16 + n16) * kBlockBytes + lds_part<128>(n16, j) * 16;
+  uint32_t w_lds = base + 2 * kXStage + (wn * TN * 16 + n16) * kBlockBytes + lds_part<128>(n16, j) * 16;
   uint32_t x_lds4 = x_lds ^ 64, w_lds4 = w_lds ^ 64;
   opaque(x_lds), opaque(x_lds4), opaque(w_lds), opaque(w_lds4);
   auto read_strip = [&](int u, int r) __attribute__((always_inline)) {

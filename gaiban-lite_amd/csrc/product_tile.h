@@ -40,13 +40,15 @@ struct ProductInt8 {
   }
 };
 
-// Where 16-byte part `part` of a row of a block lies in its 128 bytes of LDS.  The LDS serves
-// a ds_read_b128 in sets of 16 lanes (0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of each half of
-// a wavefront: measured by moving one lane at a time onto another's banks); with part j of
-// row r at j ^ (r & 7), lanes (row r, part j = lane / 16) of a set fall into all sixteen slots
-// of the 256 bytes of banks (SQ_LDS_BANK_CONFLICT 0; swz128's order, made for other reads, has
-// four conflicts a read here).
-__device__ __forceinline__ int lds_part(int row, int part) { return part ^ (row & 7); }
+// Where 16-byte part `part` of a row of a block of BLOCK bytes (128 or a multiple of 256)
+// lies in the row's bytes of LDS.  The LDS serves a ds_read_b128 in sets of 16 lanes (0-3,
+// 12-15, 20-27 and 4-11, 16-19, 28-31 of each half of a wavefront: measured by moving one
+// lane at a time onto another's banks); with part j of row r at j ^ (r & 7), for rows of
+// whole 256 bytes j ^ (r & 15), lanes (row r, part j = lane / 16) of a set fall into all
+// sixteen slots of the 256 bytes of banks (SQ_LDS_BANK_CONFLICT 0; swz128's order, made for
+// other reads, has four conflicts a read here).
+template <int BLOCK>
+__device__ __forceinline__ int lds_part(int row, int part) { return part ^ (row & (BLOCK == 128 ? 7 : 15)); }
 
 struct ProductParams {
   const uint8_t* x;  // activation rows of `kbytes` bytes
@@ -187,15 +189,15 @@ __device__ __forceinline__ uint32_t w_row_offset(const ProductParams& p, int tn,
 
 // The workgroup's finished tile to the output, through `lds` (TOK rows of all its output
 // channels) so that whole rows are stored: 16-byte part q of row r is kept at
-// q ^ (r mod parts).  Every wavefront has read its last fragments from `lds`.
-template <class Op, int TOK, int TM, int TN, int WM, int WN, bool GROUPED, bool SWIGLU>
+// q ^ (r mod parts).  Every wavefront has read its last fragments from `lds`; of WK wavefronts
+// that shared a tile's K the first has the sums.
+template <class Op, int TOK, int TM, int TN, int WM, int WN, int WK, bool GROUPED, bool SWIGLU>
 __device__ __forceinline__ void store_tile(const ProductParams& p, const typename Op::Acc (&acc)[TN][TM],
                                            uint8_t* lds, const TileRows<TOK>& rows, int tm, int tn, int expert) {
-  constexpr int kWaves = WM * WN;
   constexpr int kOutStrips = SWIGLU ? TN / 2 : TN;  // a wavefront's strips of output channels
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN;
+  const int wm = wave / WN % WM;
   const int wn = wave % WN;
   const int n16 = lane & 15;
   const int j = lane >> 4;
@@ -217,6 +219,7 @@ __device__ __forceinline__ void store_tile(const ProductParams& p, const typenam
   }
 #pragma unroll
   for (int c = 0; c < TM; ++c) {
+    if (WK > 1 && wave >= WM * WN) break;
     const int row = (c * WM + wm) * 16 + n16;
     const int id = rows.id[row];
     const float factor = rows.factor[row];
@@ -247,7 +250,7 @@ __device__ __forceinline__ void store_tile(const ProductParams& p, const typenam
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < TOK * kParts; i += 64 * kWaves) {
+  for (int i = threadIdx.x; i < TOK * kParts; i += 64 * WM * WN * WK) {
     const int row = i / kParts, q = i % kParts;
     const int ch = tn * (kParts * 8) + q * 8;
     const int id = rows.id[row];
@@ -258,30 +261,40 @@ __device__ __forceinline__ void store_tile(const ProductParams& p, const typenam
   }
 }
 
-// TOK rows x CH channels of WM x WN wavefronts, K in blocks of 128 bytes through a ring
-// of S stages in LDS.  buffer_load ... lds copies a stage (16-byte parts as lds_part says); the copies of block kb + S - 1 are issued behind the barrier of block
-// kb, when every wavefront has read block kb - 1 out of the stage they refill, so S - 2
-// blocks are in flight while one is computed.  Wavefront (wm, wn) owns token columns
-// c * WM + wm (16 rows each; interleaved, so that a partly filled tile loads the
-// wavefronts alike) and strips wn * TN .. of the tile (16 channels each).  With SwiGLU a
-// wavefront's first TN / 2 strips are gate channels and the others the same up channels.
-template <class Op, int TOK, int CH, int WM, int WN, int S, bool GROUPED, bool SWIGLU>
-__global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParams p) {
-  constexpr int kWaves = WM * WN;
+// Few rows, where the weights' stream is the bound, and small dense calls: TOK rows x CH
+// channels per workgroup, K in blocks of 128 * WK bytes through a ring of S stages in LDS.
+// buffer_load ... lds copies a stage (16-byte parts as lds_part says); the copies of block
+// kb + S - 1 are issued behind the barrier of block kb, when every wavefront has read block
+// kb - 1 out of the stage they refill, so S - 2 blocks are in flight while one is computed.
+// Wavefront (wk, wm, wn) takes the wk-th 128 bytes of every block for token columns
+// c * WM + wm (16 rows each; interleaved, so that a partly filled tile loads the wavefronts
+// alike) and strips wn * TN .. of the tile (16 channels each); the WK partial sums are added
+// in that order.  With SwiGLU a wavefront's first TN / 2 strips are gate channels and the
+// others the same up channels.
+template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool GROUPED, bool SWIGLU>
+__global__ __launch_bounds__(64 * WM * WN * WK) void product_tile_kernel(ProductParams p) {
+  constexpr int kWaves = WM * WN * WK;
   constexpr int TM = TOK / 16 / WM;
   constexpr int TN = CH / 16 / WN;
-  constexpr int kStage = (TOK + CH) * kBlockBytes;
+  constexpr int kBlock = 128 * WK;       // K bytes of a row per block
+  constexpr int kLanes = 8 * WK;         // lanes that copy a row of a block
+  constexpr int kRowsPerCopy = 64 / kLanes;
+  constexpr int kStage = (TOK + CH) * kBlock;
   constexpr int kOutStrips = SWIGLU ? TN / 2 : TN;  // a wavefront's strips of output channels
+  constexpr int kPartial = TN * TM * 1024;          // a wavefront's sums
+  static_assert(WK == 1 || WK == 2 || WK == 4 || WK == 8, "whole rows per copy");
   static_assert(TM * 16 * WM == TOK && TN * 16 * WN == CH, "whole strips and columns per wavefront");
   static_assert(!SWIGLU || TN % 2 == 0, "gate and up strips in one wavefront");
-  static_assert(CH / 8 % kWaves == 0, "every wavefront issues the same weight copies");
+  static_assert(CH / kRowsPerCopy % kWaves == 0, "every wavefront issues the same weight copies");
   static_assert(TOK * kOutStrips * 16 * WN * 2 <= S * kStage, "the output tile fits the ring");
-  __shared__ __attribute__((aligned(16))) uint8_t ring[S * kStage];
+  static_assert((WK - 1) * WM * WN * kPartial <= S * kStage, "the partial sums fit the ring");
+  __shared__ __attribute__((aligned(256))) uint8_t ring[S * kStage];
   __shared__ TileRows<TOK> rows;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN;
+  const int wk = wave / (WM * WN);
+  const int wm = wave / WN % WM;
   const int wn = wave % WN;
   const int n16 = lane & 15;
   const int j = lane >> 4;
@@ -305,8 +318,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
     const int per_xcd = (items + kTileXcds - 1) / kTileXcds;
     const int item = (blockIdx.x % kTileXcds) * per_xcd + blockIdx.x / kTileXcds;
     if (item >= items) return;
-    tm = item / p.tiles_n;
-    tn = item % p.tiles_n;
+    tm = item % p.tiles_m;
+    tn = item / p.tiles_m;
     const int64_t row0 = (int64_t)tm * TOK;
     valid = (int)(p.rows - row0 < TOK ? p.rows - row0 : TOK);
     xbase += row0 * p.kbytes;
@@ -319,34 +332,36 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   const __amdgpu_buffer_rsrc_t w_rsrc =
       __builtin_amdgcn_make_buffer_rsrc((void*)wbase, (short)0, (int)((int64_t)p.n * p.kbytes), kTileRsrcFlags);
 
-  // copy q of a stage fills its rows 8 q .. 8 q + 7 (tokens, then weights)
-  constexpr int kXCopies = (TOK / 8 + kWaves - 1) / kWaves;  // the last ones may repeat a row group
-  constexpr int kWCopies = CH / 8 / kWaves;
+  // copy q of a stage fills 1 KiB, its rows kRowsPerCopy q .. (tokens, then weights)
+  constexpr int kXGroups = TOK / kRowsPerCopy;
+  constexpr int kXCopies = (kXGroups + kWaves - 1) / kWaves;  // the last ones may repeat a group
+  constexpr int kWCopies = CH / kRowsPerCopy / kWaves;
   constexpr int kCopies = kXCopies + kWCopies;
-  uint32_t x_off[kXCopies], w_off[kWCopies];
-  uint32_t x_dst[kXCopies], w_dst[kWCopies];
+  uint32_t x_off[kXCopies], w_off[kWCopies], x_part[kXCopies], w_part[kWCopies];
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(&ring[0]));
-  // Every copy of a lane is of the same 16-byte part.  Bytes past the end of K, and whole
-  // blocks past it (the ring runs on without a branch), are read out of range: zeros.
-  const uint32_t part = lds_part(lane >> 3, lane & 7) * 16;
-  const int last = p.kblocks - 1;
-  const uint32_t tail = p.kbytes - last * kBlockBytes;  // bytes of the last block: 16 .. 128
-  auto limit = [&](int kb) { return kb < last ? kBlockBytes : (kb == last ? tail : 0); };
+  // Bytes past the end of K, and whole blocks past it (the ring runs on without a branch),
+  // are read out of range: zeros.
+  const int kblocks = (p.kbytes + kBlock - 1) / kBlock;
+  const int last = kblocks - 1;
+  const uint32_t tail = p.kbytes - last * kBlock;  // bytes of the last block
+  auto limit = [&](int kb) { return kb < last ? (uint32_t)kBlock : (kb == last ? tail : 0); };
 #pragma unroll
   for (int i = 0; i < kWCopies; ++i) {
-    const int q = wave + kWaves * i;
-    w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, q * 8 + (lane >> 3)) + part;
-    w_dst[i] = __builtin_amdgcn_readfirstlane(base + TOK * kBlockBytes + q * 1024);
+    const int row = (wave + kWaves * i) * kRowsPerCopy + lane / kLanes;
+    w_part[i] = lds_part<kBlock>(row, lane % kLanes) * 16;
+    w_off[i] = w_row_offset<CH, TN, WN, SWIGLU>(p, tn, row) + w_part[i];
   }
   auto copy_w = [&](int kb, int stage) {
 #pragma unroll
     for (int i = 0; i < kWCopies; ++i)
-      lds_copy16(w_rsrc, w_dst[i] + stage * kStage, part < limit(kb) ? w_off[i] : kTileOob, min(kb, last) * kBlockBytes);
+      lds_copy16(w_rsrc, base + stage * kStage + TOK * kBlock + (wave + kWaves * i) * 1024,
+                 w_part[i] < limit(kb) ? w_off[i] : kTileOob, min(kb, last) * kBlock);
   };
   auto copy_x = [&](int kb, int stage) {
 #pragma unroll
     for (int i = 0; i < kXCopies; ++i)
-      lds_copy16(x_rsrc, x_dst[i] + stage * kStage, part < limit(kb) ? x_off[i] : kTileOob, min(kb, last) * kBlockBytes);
+      lds_copy16(x_rsrc, base + stage * kStage + (wave + kWaves * i) % kXGroups * 1024,
+                 x_part[i] < limit(kb) ? x_off[i] : kTileOob, min(kb, last) * kBlock);
   };
   // the first weights do not wait for the rows' ids
 #pragma unroll
@@ -356,9 +371,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   valid = rows.rows();
 #pragma unroll
   for (int i = 0; i < kXCopies; ++i) {
-    const int q = (wave + kWaves * i) % (TOK / 8);
-    x_off[i] = x_row_offset<GROUPED>(p, rows.id[q * 8 + (lane >> 3)]) + part;
-    x_dst[i] = __builtin_amdgcn_readfirstlane(base + q * 1024);
+    const int row = (wave + kWaves * i) % kXGroups * kRowsPerCopy + lane / kLanes;
+    x_part[i] = lds_part<kBlock>(row, lane % kLanes) * 16;
+    x_off[i] = x_row_offset<GROUPED>(p, rows.id[row]) + x_part[i];
   }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) copy_x(s, s);
@@ -372,9 +387,10 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   // the columns of this wavefront that hold rows
   const int columns = (valid + 15) >> 4;
   const int mine = columns > wm ? (columns - wm + WM - 1) / WM : 0;
+  const int part0 = lds_part<kBlock>(n16, wk * 8 + j) * 16, part1 = lds_part<kBlock>(n16, wk * 8 + 4 + j) * 16;
 
   int stage = 0;
-  for (int kb = 0; kb < p.kblocks; ++kb) {
+  for (int kb = 0; kb < kblocks; ++kb) {
     // this wavefront's copies of block kb have landed (the first S - 1 blocks' weights were
     // copied ahead of their rows)
     if (kb < S - 2) lds_dma_wait_keep<(S - 2) * kXCopies>();
@@ -384,17 +400,17 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
     copy_x(kb + S - 1, refill);
     copy_w(kb + S - 1, refill);
     const uint8_t* xs = &ring[stage * kStage];
-    const uint8_t* ws = xs + TOK * kBlockBytes;
+    const uint8_t* ws = xs + TOK * kBlock;
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
+      const int part = d == 0 ? part0 : part1;
       u32x4 wf[TN];
 #pragma unroll
-      for (int r = 0; r < TN; ++r)
-        wf[r] = load16(ws + ((wn * TN + r) * 16 + n16) * kBlockBytes + lds_part(n16, 4 * d + j) * 16);
+      for (int r = 0; r < TN; ++r) wf[r] = load16(ws + ((wn * TN + r) * 16 + n16) * kBlock + part);
 #pragma unroll
       for (int c = 0; c < TM; ++c) {
         if (c >= mine) continue;
-        const u32x4 xf = load16(xs + ((c * WM + wm) * 16 + n16) * kBlockBytes + lds_part(n16, 4 * d + j) * 16);
+        const u32x4 xf = load16(xs + ((c * WM + wm) * 16 + n16) * kBlock + part);
 #pragma unroll
         for (int r = 0; r < TN; ++r) acc[r][c] = Op::mfma(wf[r], xf, acc[r][c]);
       }
@@ -404,7 +420,28 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductParam
   lds_dma_wait_all();
   __syncthreads();  // every wavefront has read its last fragments and its copies have landed
 
-  store_tile<Op, TOK, TM, TN, WM, WN, GROUPED, SWIGLU>(p, acc, ring, rows, tm, tn, expert);
+  if constexpr (WK > 1) {
+    typedef typename Op::Acc Acc;
+    Acc* partial = reinterpret_cast<Acc*>(ring);
+    if (wk > 0) {
+#pragma unroll
+      for (int r = 0; r < TN; ++r)
+#pragma unroll
+        for (int c = 0; c < TM; ++c) partial[((wave - WM * WN) * TN * TM + r * TM + c) * 64 + lane] = acc[r][c];
+    }
+    __syncthreads();
+    if (wk == 0) {
+#pragma unroll
+      for (int k = 0; k < WK - 1; ++k)
+#pragma unroll
+        for (int r = 0; r < TN; ++r)
+#pragma unroll
+          for (int c = 0; c < TM; ++c)
+            acc[r][c] += partial[((k * WM * WN + wave) * TN * TM + r * TM + c) * 64 + lane];
+    }
+    __syncthreads();  // before the output tile takes their place
+  }
+  store_tile<Op, TOK, TM, TN, WM, WN, WK, GROUPED, SWIGLU>(p, acc, ring, rows, tm, tn, expert);
 }
 
 }  // namespace dsv4
