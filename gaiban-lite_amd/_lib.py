@@ -187,7 +187,7 @@ def call(name: str, *args) -> None:
     DSV4MOE_EHIP -> Dsv4MoEError.
     """
 
-    rc = getattr(load(), name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc == DSV4MOE_OK:
         return
     msg = last_error()

@@ -56,10 +56,10 @@ class GroupedPlan:
     block_size: int
     swiglu: bool = False
     per_slot: bool = False
+    capacity: int = 0  # of the alignment's sorted_token_ids
 
     slots = property(lambda self: self.tokens * self.topk)
     rows = property(lambda self: self.slots if self.per_slot else self.tokens)
-    capacity = property(lambda self: max_padded_tokens(self.slots, self.experts, self.block_size))
     activation_shape = property(lambda self: (self.rows, self.k))
     activation_scale_shape = property(lambda self: (self.rows,))
     weight_shape = property(lambda self: (self.experts, self.n, self.k))
@@ -88,20 +88,18 @@ def make_grouped_plan(tokens: int, topk: int, experts: int, n: int, k: int, *, b
     if k % 8:
         raise ValueError(f"k={k} is not a multiple of 8")
     return GroupedPlan(tokens=tokens, topk=topk, experts=experts, n=n, k=k, block_size=block_size, swiglu=swiglu,
-                       per_slot=per_slot)
+                       per_slot=per_slot, capacity=max_padded_tokens(tokens * topk, experts, block_size))
 
 
-def _check_plan(plan: GroupedPlan, x, weight, sorted_token_ids) -> None:
+def _check_plan(plan: GroupedPlan, x, weight, sorted_token_ids, dtype: torch.dtype) -> None:
     if not isinstance(plan, GroupedPlan):
         raise TypeError(f"plan: expected GroupedPlan, got {type(plan).__name__}")
     for name, value, shape in (("activation", x, plan.activation_shape), ("weight", weight, plan.weight_shape),
                                ("sorted_token_ids", sorted_token_ids, (plan.capacity,))):
-        if not isinstance(value, torch.Tensor):
-            raise TypeError(f"{name}: expected a tensor, got {type(value).__name__}")
-        if value.shape != shape:
-            raise ValueError(f"{name}: shape {tuple(value.shape)}, the plan needs {shape}")
-    if weight.dtype not in WEIGHT_DTYPES:
-        raise TypeError(f"weight: element type {weight.dtype} is not bfloat16 or int8")
+        if not isinstance(value, torch.Tensor) or value.shape != shape:
+            C.tensor(name, value, shape=shape)
+    if weight.dtype is not dtype:
+        C.tensor("weight", weight, dtype=dtype)
 
 
 def grouped_linear_into(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, *, plan: GroupedPlan,
@@ -111,8 +109,7 @@ def grouped_linear_into(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor
     """The product over bf16 weights [experts, n, k]: ``x`` bf16
     ``plan.activation_shape``, ``out`` bf16 ``plan.output_shape``."""
 
-    _check_plan(plan, x, weight, sorted_token_ids)
-    C.tensor("weight", weight, dtype=torch.bfloat16)
+    _check_plan(plan, x, weight, sorted_token_ids, torch.bfloat16)
     ops.grouped_gemm_into(x, weight, out, tokens=plan.tokens, topk=plan.topk, sorted_token_ids=sorted_token_ids,
                           expert_ids=expert_ids, num_tokens_post_padded=num_tokens_post_padded,
                           block_size=plan.block_size, per_slot=plan.per_slot, swiglu=plan.swiglu,
@@ -128,8 +125,7 @@ def grouped_int8_gemm_into(activation: torch.Tensor, activation_scale: torch.Ten
     [experts, n], of activations quantised before (int8 codes with one fp32
     scale per row: ``int8_linear.activation_quant_into``)."""
 
-    _check_plan(plan, activation, weight, sorted_token_ids)
-    C.tensor("weight", weight, dtype=torch.int8)
+    _check_plan(plan, activation, weight, sorted_token_ids, torch.int8)
     ops.grouped_gemm_into(activation, weight, out, tokens=plan.tokens, topk=plan.topk,
                           sorted_token_ids=sorted_token_ids, expert_ids=expert_ids,
                           num_tokens_post_padded=num_tokens_post_padded, block_size=plan.block_size,
@@ -145,8 +141,7 @@ def grouped_int8_linear_into(x: torch.Tensor, weight: torch.Tensor, weight_scale
     """The quantiser over ``x`` (bf16, fp16 or fp32) into ``quantized`` int8
     and ``scale`` fp32 (one per row), then ``grouped_int8_gemm_into``."""
 
-    _check_plan(plan, x, weight, sorted_token_ids)
-    C.tensor("weight", weight, dtype=torch.int8)
+    _check_plan(plan, x, weight, sorted_token_ids, torch.int8)
     ops.grouped_gemm_into(x, weight, out, tokens=plan.tokens, topk=plan.topk, sorted_token_ids=sorted_token_ids,
                           expert_ids=expert_ids, num_tokens_post_padded=num_tokens_post_padded,
                           block_size=plan.block_size, per_slot=plan.per_slot, swiglu=plan.swiglu,

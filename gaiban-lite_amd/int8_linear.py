@@ -71,14 +71,10 @@ def make_gemm_plan(m: int, n: int, k: int) -> Int8GemmPlan:
 def _check_plan(plan: Int8GemmPlan, activation, weight=None) -> None:
     if not isinstance(plan, Int8GemmPlan):
         raise TypeError(f"plan: expected Int8GemmPlan, got {type(plan).__name__}")
-    for name, value, shape in (("activation", activation, plan.activation_shape),
-                               ("weight", weight, plan.weight_shape)):
-        if name == "weight" and weight is None:
-            continue
-        if not isinstance(value, torch.Tensor):
-            raise TypeError(f"{name}: expected a tensor, got {type(value).__name__}")
-        if value.shape != shape:
-            raise ValueError(f"{name}: shape {tuple(value.shape)}, the plan needs {shape}")
+    if not isinstance(activation, torch.Tensor) or activation.shape != (plan.m, plan.k):
+        C.tensor("activation", activation, shape=plan.activation_shape)
+    if weight is not None and (not isinstance(weight, torch.Tensor) or weight.shape != (plan.n, plan.k)):
+        C.tensor("weight", weight, shape=plan.weight_shape)
 
 
 def activation_quant_into(x: torch.Tensor, quantized_out: torch.Tensor, scale_out: torch.Tensor, *,

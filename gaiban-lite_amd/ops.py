@@ -724,11 +724,21 @@ def _launch(device: torch.device, name: str, *args) -> None:
     """``name(*args, stream)`` on ``device``'s current stream, with ``device``
     current for the launch (it may differ from the caller's)."""
 
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _lib.current_stream(device))
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
         return
     with torch.cuda.device(device):
         call(name, *args, _lib.current_stream(device))
+
+
+def _require(name, t, dtype, shape, device) -> None:
+    """``_check`` of a device tensor, the passing case first: a decode step's
+    call is short against its checks."""
+
+    if not (type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and t.device == device
+            and t.is_cuda and t.is_contiguous()):
+        _check(name, t, dtype=dtype, shape=shape, device=device)
 
 
 def _quant_dtype(x: torch.Tensor) -> int:
@@ -748,10 +758,10 @@ def act_quant_int8_into(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -
     code = _quant_dtype(x)
     m, k = x.shape
     dev = x.device
-    _check("x", x, dtype=x.dtype, device=dev)
-    _check("quantized_out", q, dtype=torch.int8, shape=(m, k), device=dev)
-    _check("scale_out", scale, dtype=torch.float32, shape=(m,), device=dev)
-    _launch(dev, "dsv4moe_act_quant_int8", ptr(x), code, m, k, ptr(q), ptr(scale))
+    _require("x", x, x.dtype, (m, k), dev)
+    _require("quantized_out", q, torch.int8, (m, k), dev)
+    _require("scale_out", scale, torch.float32, (m,), dev)
+    _launch(dev, "dsv4moe_act_quant_int8", x.data_ptr(), code, m, k, q.data_ptr(), scale.data_ptr())
 
 
 def int8_gemm_into(a: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
@@ -764,12 +774,13 @@ def int8_gemm_into(a: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, ws:
     m, k = a.shape
     n = wq.shape[0]
     dev = a.device
-    _check("activation", a, dtype=torch.int8, device=dev)
-    _check("activation_scale", a_scale, dtype=torch.float32, shape=(m,), device=dev)
-    _check("weight", wq, dtype=torch.int8, shape=(n, k), device=dev)
-    _check("weight_scale", ws, dtype=torch.bfloat16, shape=(n,), device=dev)
-    _check("out", out, dtype=torch.bfloat16, shape=(m, n), device=dev)
-    _launch(dev, "dsv4moe_int8_gemm", ptr(a), ptr(a_scale), m, n, k, ptr(wq), ptr(ws), ptr(out))
+    _require("activation", a, torch.int8, (m, k), dev)
+    _require("activation_scale", a_scale, torch.float32, (m,), dev)
+    _require("weight", wq, torch.int8, (n, k), dev)
+    _require("weight_scale", ws, torch.bfloat16, (n,), dev)
+    _require("out", out, torch.bfloat16, (m, n), dev)
+    _launch(dev, "dsv4moe_int8_gemm", a.data_ptr(), a_scale.data_ptr(), m, n, k, wq.data_ptr(), ws.data_ptr(),
+            out.data_ptr())
 
 
 def int8_linear_into(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out: torch.Tensor, q: torch.Tensor,
@@ -784,13 +795,14 @@ def int8_linear_into(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, out: t
     m, k = x.shape
     n = wq.shape[0]
     dev = x.device
-    _check("x", x, dtype=x.dtype, device=dev)
-    _check("weight", wq, dtype=torch.int8, shape=(n, k), device=dev)
-    _check("weight_scale", ws, dtype=torch.bfloat16, shape=(n,), device=dev)
-    _check("out", out, dtype=torch.bfloat16, shape=(m, n), device=dev)
-    _check("quantized", q, dtype=torch.int8, shape=(m, k), device=dev)
-    _check("scale", scale, dtype=torch.float32, shape=(m,), device=dev)
-    _launch(dev, "dsv4moe_int8_linear", ptr(x), code, m, n, k, ptr(wq), ptr(ws), ptr(q), ptr(scale), ptr(out))
+    _require("x", x, x.dtype, (m, k), dev)
+    _require("weight", wq, torch.int8, (n, k), dev)
+    _require("weight_scale", ws, torch.bfloat16, (n,), dev)
+    _require("out", out, torch.bfloat16, (m, n), dev)
+    _require("quantized", q, torch.int8, (m, k), dev)
+    _require("scale", scale, torch.float32, (m,), dev)
+    _launch(dev, "dsv4moe_int8_linear", x.data_ptr(), code, m, n, k, wq.data_ptr(), ws.data_ptr(), q.data_ptr(),
+            scale.data_ptr(), out.data_ptr())
 
 
 def grouped_gemm_into(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, tokens: int, topk: int,
@@ -817,30 +829,31 @@ def grouped_gemm_into(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, to
     int8 = w.dtype == torch.int8
     if quantized is not None:
         x_code = _quant_dtype(x)
-        _check("quantized", quantized, dtype=torch.int8, shape=(rows, k), device=dev)
-        _check("x", x, dtype=x.dtype, shape=(rows, k), device=dev)
+        _require("quantized", quantized, torch.int8, (rows, k), dev)
+        _require("x", x, x.dtype, (rows, k), dev)
     else:
-        _check("x", x, dtype=torch.int8 if int8 else torch.bfloat16, shape=(rows, k), device=dev)
-    _check("weight", w, dtype=torch.int8 if int8 else torch.bfloat16, device=dev)
-    _check("out", out, dtype=torch.bfloat16, shape=(slots, n // 2 if swiglu else n), device=dev)
-    _check("sorted_token_ids", sorted_token_ids, dtype=torch.int32, device=dev)
+        _require("x", x, torch.int8 if int8 else torch.bfloat16, (rows, k), dev)
+    _require("weight", w, torch.int8 if int8 else torch.bfloat16, (experts, n, k), dev)
+    _require("out", out, torch.bfloat16, (slots, n // 2 if swiglu else n), dev)
     capacity = sorted_token_ids.numel()
-    _check("expert_ids", expert_ids, dtype=torch.int32, shape=(-(-capacity // block_size),), device=dev)
-    _check("num_tokens_post_padded", num_tokens_post_padded, dtype=torch.int32, shape=(1,), device=dev)
+    _require("sorted_token_ids", sorted_token_ids, torch.int32, (capacity,), dev)
+    _require("expert_ids", expert_ids, torch.int32, (-(-capacity // block_size),), dev)
+    _require("num_tokens_post_padded", num_tokens_post_padded, torch.int32, (1,), dev)
     if route_weights is not None:
-        _check("route_weights", route_weights, dtype=torch.float32, shape=(tokens, topk), device=dev)
+        _require("route_weights", route_weights, torch.float32, (tokens, topk), dev)
     if int8:
-        _check("activation_scale", x_scale, dtype=torch.float32, shape=(rows,), device=dev)
-        _check("weight_scale", ws, dtype=torch.bfloat16, shape=(experts, n), device=dev)
+        _require("activation_scale", x_scale, torch.float32, (rows,), dev)
+        _require("weight_scale", ws, torch.bfloat16, (experts, n), dev)
     elif x_scale is not None or ws is not None or quantized is not None:
         raise ValueError("only int8 weights take scales")
-    args = (tokens, topk, int(bool(per_slot)), n, k, experts, ptr(w))
-    rest = (ptr(sorted_token_ids), capacity, ptr(expert_ids), ptr(num_tokens_post_padded), block_size,
-            int(bool(swiglu)), float(clamp_limit), ptr(route_weights))
+    args = (tokens, topk, per_slot, n, k, experts, w.data_ptr())
+    rest = (sorted_token_ids.data_ptr(), capacity, expert_ids.data_ptr(), num_tokens_post_padded.data_ptr(),
+            block_size, swiglu, clamp_limit, None if route_weights is None else route_weights.data_ptr())
     if quantized is not None:
-        _launch(dev, "dsv4moe_grouped_int8_linear", ptr(x), x_code, *args, ptr(ws), *rest, ptr(quantized),
-                ptr(x_scale), ptr(out))
+        _launch(dev, "dsv4moe_grouped_int8_linear", x.data_ptr(), x_code, *args, ws.data_ptr(), *rest,
+                quantized.data_ptr(), x_scale.data_ptr(), out.data_ptr())
     elif int8:
-        _launch(dev, "dsv4moe_grouped_int8_gemm", ptr(x), ptr(x_scale), *args, ptr(ws), *rest, ptr(out))
+        _launch(dev, "dsv4moe_grouped_int8_gemm", x.data_ptr(), x_scale.data_ptr(), *args, ws.data_ptr(), *rest,
+                out.data_ptr())
     else:
-        _launch(dev, "dsv4moe_grouped_gemm", ptr(x), *args, *rest, ptr(out))
+        _launch(dev, "dsv4moe_grouped_gemm", x.data_ptr(), *args, *rest, out.data_ptr())
