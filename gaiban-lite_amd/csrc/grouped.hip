@@ -1,9 +1,27 @@
 // Linears grouped by expert over bf16 or int8 weights [E, N, K]: slot i's activation row
 // times its expert's weights, the slots sorted by expert in padded blocks (dsv4moe_align).
+#include <algorithm>
+#include <cmath>
+
 #include "product_gemm.h"
 #include "../../include/dsv4moe.h"
 
 namespace dsv4 {
+
+// Tiles of `tok` rows per expert with slots, estimated from the mean (the routes are on the
+// device).
+static double tiles_per_expert(const ProductParams& p, int tok) {
+  const double used = p.slots < p.experts ? p.slots : p.experts;
+  const double share = p.slots / used / tok;
+  return share <= 0.85 ? 1.0 : share + 0.5;
+}
+
+// Weights that one tile reads, in whole lines, and more of them than the 256 MB cache in front
+// of HBM would still hold when a call after the next reads them again.
+static bool weights_once(const ProductParams& p, int tok) {
+  const double used = p.slots < p.experts ? p.slots : p.experts;
+  return tiles_per_expert(p, tok) == 1.0 && p.kbytes % 128 == 0 && used * p.n * p.kbytes > 96e6;
+}
 
 template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool SWIGLU>
 static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
@@ -11,8 +29,11 @@ static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
   p.tiles_m = p.blocks;
   p.tiles_n = (p.n + CH - 1) / CH;
   const dim3 grid((unsigned)(p.blocks * p.tiles_n));
-  hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU>), grid, dim3(64 * WM * WN * WK), 0, stream,
-                     p);
+  const dim3 block(64 * WM * WN * WK);
+  if (weights_once(p, TOK))
+    hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, false>), grid, block, 0, stream, p);
 }
 
 template <class Op, int TOK, int CH, int WM, int WN, bool SWIGLU>
@@ -21,16 +42,53 @@ static void launch_grouped_gemm(ProductParams p, hipStream_t stream) {
   p.tiles_n = (p.n + CH - 1) / CH;
   const int64_t items = ((int64_t)p.blocks * p.tiles_n + kTileXcds - 1) / kTileXcds * kTileXcds;
   const dim3 grid((unsigned)(items < kGemmCus ? items : kGemmCus));
-  hipLaunchKernelGGL((product_gemm_kernel<Op, TOK, CH, WM, WN, true, SWIGLU>), grid, dim3(512), 0, stream, p);
+  if (weights_once(p, TOK))
+    hipLaunchKernelGGL((product_gemm_kernel<Op, TOK, CH, WM, WN, true, SWIGLU, true>), grid, dim3(512), 0, stream, p);
+  else
+    hipLaunchKernelGGL((product_gemm_kernel<Op, TOK, CH, WM, WN, true, SWIGLU, false>), grid, dim3(512), 0, stream, p);
 }
 
+// The kernel of a call.  Blocks of up to 16 slots (few tokens): 16 x 32 tiles, 512 bytes of K
+// a stage, which stream the weights at 6.3 TB/s (64 tokens, 256 experts, N=4096, K=2048: 530
+// us against 545-575 with 64 channels and 128 bytes).  Blocks of 32: 128 channels where there
+// are workgroups enough (1000 tokens over 256 experts, N=K=4096 1556 us against 1672 with 64;
+// 60 tokens x 2 over 8 experts 60 us against 53).  Longer blocks: the least time by a model --
+// a start, then a CU's share of the tiles times (K blocks x time per block + end), or the
+// experts' weights at 5.9 TB/s where that is more; the tiles per expert are estimated from
+// the mean (the routes are on the device).  us, bf16, model / measured: 5000 tokens x 4 over
+// 64 experts, N=K=1024: 128 x 256 62 / 58, 256 x 256 63 / 65, 128 x 128 65 / 68, 64 x 128 77 /
+// 80, 64 x 64 96 / 92; 200 x 2 over 8, N=2048, K=1024: 64 x 64 8.6 / 9.2, 64 x 128 11.3 / 10.4,
+// 128 x 128 15 / 13.
 template <class Op, bool SWIGLU>
 static void launch_grouped(const ProductParams& p, hipStream_t stream) {
-  const int per_expert = p.slots / p.experts;
-  if (per_expert >= 64) return launch_grouped_gemm<Op, 256, 256, 4, 2, SWIGLU>(p, stream);
-  if (p.block_size <= 16) launch_grouped_tile<Op, 16, 32, 1, 1, 4, 2, SWIGLU>(p, stream);
-  else if (p.block_size <= 32) launch_grouped_tile<Op, 32, 128, 1, 4, 2, 3, SWIGLU>(p, stream);
-  else launch_grouped_tile<Op, 64, 128, 2, 4, 1, 3, SWIGLU>(p, stream);
+  const double used = p.slots < p.experts ? p.slots : p.experts;
+  auto tiles = [&](int tok, int ch) { return used * tiles_per_expert(p, tok) * ((p.n + ch - 1) / ch); };
+  if (p.block_size <= 16) return launch_grouped_tile<Op, 16, 32, 1, 1, 4, 2, SWIGLU>(p, stream);
+  if (p.block_size <= 32) {
+    if (tiles(32, 128) >= 4 * kGemmCus) return launch_grouped_tile<Op, 32, 128, 1, 4, 2, 3, SWIGLU>(p, stream);
+    return launch_grouped_tile<Op, 32, 64, 1, 2, 2, 3, SWIGLU>(p, stream);
+  }
+  struct Tile {
+    int tok, ch;
+    double start, block, end;
+    void (*launch)(ProductParams, hipStream_t);
+  };
+  static const Tile kernels[] = {
+      {128, 256, 5.0, 1.0, 3.0, launch_grouped_gemm<Op, 128, 256, 2, 4, SWIGLU>},
+      {256, 256, 5.0, 1.62, 3.0, launch_grouped_gemm<Op, 256, 256, 4, 2, SWIGLU>},
+      {128, 128, 5.0, 0.47, 2.5, launch_grouped_gemm<Op, 128, 128, 4, 2, SWIGLU>},
+      {64, 128, 4.0, 0.38, 1.2, launch_grouped_tile<Op, 64, 128, 2, 4, 1, 3, SWIGLU>},
+      {64, 64, 4.0, 0.25, 0.6, launch_grouped_tile<Op, 64, 64, 2, 2, 1, 3, SWIGLU>},
+  };
+  const double read = used * p.n * p.kbytes / 5.9e6;
+  const Tile* best = nullptr;
+  double least = 0.0;
+  for (const Tile& t : kernels) {
+    const double rounds = std::ceil(tiles(t.tok, t.ch) / kGemmCus);
+    const double time = std::max(read, t.start + rounds * (p.kblocks * t.block + t.end));
+    if (best == nullptr || time < least) best = &t, least = time;
+  }
+  best->launch(p, stream);
 }
 
 }  // namespace dsv4

@@ -153,6 +153,8 @@ static void launch_quant(const void* x, int64_t m, int k, int8_t* q, float* scal
 // rows x 256 bytes at a time, into kFewStages stages of its own, so that nothing but the end
 // of a strip needs a barrier: there the eight partial sums (exact, int32) are added.  A lane
 // whose token does not exist reads another's codes, for a column that nothing stores.
+// Weights from HBM, us, against the quantiser and a tile kernel: N=K=4096 M=1 8.0 / 13.8, M=8
+// 10.8 / 14.3, N=16384 M=1 17.3 (3.9 TB/s) / 21.6, N=4096 K=2048 M=16 9.0 / 10.1.
 struct FewParams {
   const void* x;
   int m, n, k;
@@ -161,10 +163,9 @@ struct FewParams {
   uint16_t* out;
 };
 constexpr int kFewWaves = 8;
-constexpr int kFewStages = 3;
 constexpr int kFewSlice = 256;                      // K bytes of a wavefront per stage
 constexpr int kFewRound = kFewWaves * kFewSlice;    // K bytes of a workgroup per stage
-constexpr int kFewRing = kFewWaves * kFewStages * 16 * kFewSlice;
+constexpr int kFewStages = 3;                       // (four measured the same)
 constexpr int kFewCodes = 44 * 1024;                // all tokens' codes
 
 static int64_t few_code_bytes(int64_t m, int64_t k) { return m * ((k + kFewRound - 1) / kFewRound * kFewRound); }
@@ -177,7 +178,7 @@ __device__ __forceinline__ void lds_wait_all() {
 
 template <int X>
 __global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t lds[kFewRing];
+  __shared__ __attribute__((aligned(256))) uint8_t lds[kFewWaves * kFewStages * 16 * kFewSlice];
   __shared__ __attribute__((aligned(256))) uint8_t codes[kFewCodes];  // [m][rounds * kFewRound]
   __shared__ i32x4 sums[2][kFewWaves][64];
   __shared__ uint32_t amax_of[16][kFewWaves];
@@ -211,28 +212,31 @@ __global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
 #pragma unroll
   for (int s = 0; s < kFewStages - 1; ++s) copy(s, s);
 
-  // quantise: each row by all threads, 8 values at a time
+  // quantise: a row by 8, 4, 2 or 1 wavefronts, 8 values of a lane at a time
+  const int per_row = p.m == 1 ? 8 : (p.m == 2 ? 4 : (p.m <= 4 ? 2 : 1));
   const int chunks = p.k / 8;
-  for (int r = 0; r < p.m; ++r) {
+  const int c0 = wave % per_row * 64 + lane;
+  for (int r = wave / per_row; r < p.m; r += kFewWaves / per_row) {
     uint32_t amax = 0;
-    for (int c = threadIdx.x; c < chunks; c += 512) {
+#pragma unroll 4
+    for (int c = c0; c < chunks; c += 64 * per_row) {
       float f[8];
       load8_as_float<X>(p.x, (int64_t)r * p.k + c * 8, f);
       amax = max_magnitude(amax, f);
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, off, 64));
-    if (lane == 0) amax_of[r][wave] = amax;
+    if (lane == 0) amax_of[r][wave % per_row] = amax;
   }
   __syncthreads();
-  for (int r = 0; r < p.m; ++r) {
+  for (int r = wave / per_row; r < p.m; r += kFewWaves / per_row) {
     uint32_t amax = 0;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) amax = max(amax, amax_of[r][w]);
+    for (int w = 0; w < per_row; ++w) amax = max(amax, amax_of[r][w]);
     const float s = int8_row_scale(amax);
     const float inv = 1.0f / s;
-    if (threadIdx.x == 0) scale_of[r] = s;
-    for (int c = threadIdx.x; c < code_row / 8; c += 512) {
+    if (c0 == 0) scale_of[r] = s;
+#pragma unroll 4
+    for (int c = c0; c < code_row / 8; c += 64 * per_row) {
       u32x2 q = {0, 0};
       if (c < chunks) {
         float f[8];
@@ -309,8 +313,8 @@ static void launch_tile(ProductParams p, hipStream_t stream) {
   p.tiles_n = (p.n + CH - 1) / CH;
   const int items = p.tiles_m * p.tiles_n;
   const dim3 grid((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds));
-  hipLaunchKernelGGL((product_tile_kernel<ProductInt8, TOK, CH, WM, WN, WK, S, false, false>), grid, dim3(64 * WM * WN * WK), 0,
-                     stream, p);
+  hipLaunchKernelGGL((product_tile_kernel<ProductInt8, TOK, CH, WM, WN, WK, S, false, false, false>), grid,
+                     dim3(64 * WM * WN * WK), 0, stream, p);
 }
 
 template <int TOK, int CH, int WM, int WN>
@@ -319,7 +323,7 @@ static void launch_gemm(ProductParams p, hipStream_t stream) {
   p.tiles_n = (p.n + CH - 1) / CH;
   const int64_t items = ((int64_t)p.tiles_m * p.tiles_n + kTileXcds - 1) / kTileXcds * kTileXcds;
   const dim3 grid((unsigned)(items < kGemmCus ? items : kGemmCus));
-  hipLaunchKernelGGL((product_gemm_kernel<ProductInt8, TOK, CH, WM, WN, false, false>), grid, dim3(512), 0, stream, p);
+  hipLaunchKernelGGL((product_gemm_kernel<ProductInt8, TOK, CH, WM, WN, false, false, false>), grid, dim3(512), 0, stream, p);
 }
 
 // The tile with the least time by a model: a start, then its workgroups' share of tiles per

@@ -116,7 +116,7 @@ __device__ __forceinline__ void opaque(uint32_t& v) {
 // An XCD takes neighbouring items: grouped, all channel tiles of an expert's rows; dense,
 // kGemmGroup row tiles walking the channel tiles together.  Columns without rows are not
 // multiplied (grouped): COLS of the TM columns of a wavefront, chosen per tile.
-template <class Op, int TOK, int CH, int WM, int WN, bool GROUPED, bool SWIGLU>
+template <class Op, int TOK, int CH, int WM, int WN, bool GROUPED, bool SWIGLU, bool ONCE>
 __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   constexpr int kWaves = WM * WN;
   constexpr int TM = TOK / 16 / WM;
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
       lds_copy16(x_rsrc, base + u * kXStage + (wave + kWaves * i) * 1024, off, soff);
     } else {
       off += (uint32_t)(w_row(w_group(i - kXCopies)) - w_row(w_group(0))) * (uint32_t)p.kbytes;
-      lds_copy16(w_rsrc, base + 2 * kXStage + u * kWStage + w_group(i - kXCopies) * 1024, off, soff);
+      copy_weights16<ONCE>(w_rsrc, base + 2 * kXStage + u * kWStage + w_group(i - kXCopies) * 1024, off, soff);
     }
   };
 

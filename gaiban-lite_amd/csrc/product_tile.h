@@ -115,6 +115,27 @@ __device__ __forceinline__ GroupedTile grouped_tile(const ProductParams& p, int 
   return t;
 }
 
+// lds_copy16 of weights.  ONCE: by one workgroup alone, so the lines need not stay in the
+// caches (nt).  One token over 256 experts (N=K=4096) 36.6 -> 33.8 us, 64 tokens (K=2048) 549
+// -> 521, 1000 tokens 1553 -> 1460 (5.9 TB/s); weights that several tiles read lose by it (64
+// experts, 512 rows each, 585 -> 650), and so do rows that are not whole 128-byte lines, whose
+// ends two blocks share (K=1424 41 -> 46.5), and weights that the cache in front of HBM still
+// holds from the call before (a dense call over 67 MB 15.9 -> 20.0).
+template <bool ONCE>
+__device__ __forceinline__ void copy_weights16(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, uint32_t voffset,
+                                               uint32_t soffset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voffset), "s"(rsrc),
+                   "s"(__builtin_amdgcn_readfirstlane(soffset))
+                 : "memory", "m0");
+  else
+    lds_copy16(rsrc, lds, voffset, soffset);
+#endif
+}
+
 // silu(min(g, L)) * clamp(u, -L, L), or without limits where L = 0
 __device__ __forceinline__ float swiglu_value(float g, float u, float limit) {
   if (limit > 0.0f) {
@@ -271,7 +292,7 @@ __device__ __forceinline__ void store_tile(const ProductParams& p, const typenam
 // alike) and strips wn * TN .. of the tile (16 channels each); the WK partial sums are added
 // in that order.  With SwiGLU a wavefront's first TN / 2 strips are gate channels and the
 // others the same up channels.
-template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool GROUPED, bool SWIGLU>
+template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool GROUPED, bool SWIGLU, bool ONCE>
 __global__ __launch_bounds__(64 * WM * WN * WK) void product_tile_kernel(ProductParams p) {
   constexpr int kWaves = WM * WN * WK;
   constexpr int TM = TOK / 16 / WM;
@@ -354,7 +375,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void product_tile_kernel(Product
   auto copy_w = [&](int kb, int stage) {
 #pragma unroll
     for (int i = 0; i < kWCopies; ++i)
-      lds_copy16(w_rsrc, base + stage * kStage + TOK * kBlock + (wave + kWaves * i) * 1024,
+      copy_weights16<ONCE>(w_rsrc, base + stage * kStage + TOK * kBlock + (wave + kWaves * i) * 1024,
                  w_part[i] < limit(kb) ? w_off[i] : kTileOob, min(kb, last) * kBlock);
   };
   auto copy_x = [&](int kb, int stage) {
