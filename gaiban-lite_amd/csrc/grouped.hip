@@ -23,19 +23,6 @@ static bool weights_once(const ProductParams& p, int tok) {
   return tiles_per_expert(p, tok) == 1.0 && p.kbytes % 128 == 0 && used * p.n * p.kbytes > 96e6;
 }
 
-template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool SWIGLU>
-static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
-  p.tile_blocks = TOK / p.block_size;
-  p.tiles_m = p.blocks;
-  p.tiles_n = (p.n + CH - 1) / CH;
-  const dim3 grid((unsigned)(p.blocks * p.tiles_n));
-  const dim3 block(64 * WM * WN * WK);
-  if (weights_once(p, TOK))
-    hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, true>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, false>), grid, block, 0, stream, p);
-}
-
 template <class Op, int TOK, int CH, int WM, int WN, bool SWIGLU>
 static void launch_grouped_gemm(ProductParams p, hipStream_t stream) {
   p.tile_blocks = TOK / p.block_size;
@@ -46,6 +33,22 @@ static void launch_grouped_gemm(ProductParams p, hipStream_t stream) {
     hipLaunchKernelGGL((product_gemm_kernel<Op, TOK, CH, WM, WN, true, SWIGLU, true>), grid, dim3(512), 0, stream, p);
   else
     hipLaunchKernelGGL((product_gemm_kernel<Op, TOK, CH, WM, WN, true, SWIGLU, false>), grid, dim3(512), 0, stream, p);
+}
+
+template <class Op, int TOK, int CH, int WM, int WN, int WK, int S, bool SWIGLU>
+static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
+  p.tile_blocks = TOK / p.block_size;
+  p.tiles_m = p.blocks;
+  p.tiles_n = (p.n + CH - 1) / CH;
+  const dim3 block(64 * WM * WN * WK);
+  // a launch has fewer than 2^32 threads; workgroups that stay have no such limit
+  if ((int64_t)p.blocks * p.tiles_n * block.x > 0xFFFFFFFFll)
+    return launch_grouped_gemm<Op, 128, 256, 2, 4, SWIGLU>(p, stream);
+  const dim3 grid((unsigned)(p.blocks * p.tiles_n));
+  if (weights_once(p, TOK))
+    hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, false>), grid, block, 0, stream, p);
 }
 
 // The kernel of a call.  Blocks of up to 16 slots (few tokens): 16 x 32 tiles, 512 bytes of K

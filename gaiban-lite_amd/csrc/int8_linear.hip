@@ -131,8 +131,14 @@ __global__ __launch_bounds__(256) void act_quant_int8_kernel(const void* __restr
 template <int X, int LANES, int HELD>
 static void launch_quant_as(const void* x, int64_t m, int k, int8_t* q, float* scale, hipStream_t stream) {
   constexpr int kRows = 256 / LANES;
-  hipLaunchKernelGGL((act_quant_int8_kernel<X, LANES, HELD>), dim3((unsigned)((m + kRows - 1) / kRows)), dim3(256), 0,
-                     stream, x, m, k, q, scale);
+  constexpr int64_t kMost = (int64_t)kRows << 23;  // rows of a launch, which has fewer than 2^32 threads
+  constexpr int kItem = X == DSV4MOE_DTYPE_FP32 ? 4 : 2;
+  for (int64_t at = 0; at < m; at += kMost) {
+    const int64_t rows = m - at < kMost ? m - at : kMost;
+    hipLaunchKernelGGL((act_quant_int8_kernel<X, LANES, HELD>), dim3((unsigned)((rows + kRows - 1) / kRows)),
+                       dim3(256), 0, stream, static_cast<const char*>(x) + at * k * kItem, rows, k, q + at * k,
+                       scale + at);
+  }
 }
 
 // A workgroup per row, or with many short rows a wavefront: M=32768 K=2048 38 against 46 us

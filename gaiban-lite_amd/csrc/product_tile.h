@@ -136,11 +136,12 @@ __device__ __forceinline__ void copy_weights16(__amdgpu_buffer_rsrc_t rsrc, uint
 #endif
 }
 
-// silu(min(g, L)) * clamp(u, -L, L), or without limits where L = 0
+// silu(min(g, L)) * clamp(u, -L, L), or without limits where L = 0.  Comparisons, which a NaN
+// fails: fminf would turn it into L, and a row whose scale is NaN into finite numbers.
 __device__ __forceinline__ float swiglu_value(float g, float u, float limit) {
   if (limit > 0.0f) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : (u < -limit ? -limit : u);
   }
   return silu_rcp(g) * u;
 }

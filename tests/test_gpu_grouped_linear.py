@@ -304,3 +304,111 @@ def test_graph_replays_with_new_routes(int8):
         step()
         assert torch.equal(got, out), i
         check(got, *reference(data[0], data[1], ids, **ref))
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("tokens,block_size", [(3, 8), (40, 16), (200, 32), (300, 64), (20000, 64)])
+def test_a_nan_passes_the_clamp(tokens, block_size, int8):
+    """A NaN activation, gate channel or up channel is NaN in what it reaches
+    and nowhere else, whatever the limits."""
+
+    experts, half = 4, 96
+    ids = torch.randint(0, experts, (tokens, 2), device=DEV, generator=gen(11)).to(torch.int32)
+    ids[:, 0] = 1
+    _, args, kw, data, ref = make(tokens, 2, experts, 2 * half, 272, "up", int8, 12, ids=ids, block_size=block_size)
+    clean = run(args, kw, int8).clone()
+    x, w = args[0], args[1]
+    x[tokens - 1, 17] = float("nan")
+    if int8:
+        args[2][1, 5] = args[2][1, half + 40] = float("nan")
+    else:
+        w[1, 5, 3] = w[1, half + 40, 271] = float("nan")
+    out = run(args, kw, int8)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[2 * (tokens - 1):] = True
+    for ch in (5, 40):
+        bad[:, ch] |= ids.flatten() == 1
+    assert torch.isnan(out[bad]).all()
+    assert torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("tokens,topk,experts,n,k", [
+    (2048, 6, 16, 1056, 336), (4000, 6, 40, 1056, 336), (3000, 4, 64, 544, 528), (9000, 4, 24, 320, 656),
+])
+@pytest.mark.parametrize("form", FORMS)
+def test_many_rows_ragged_channels(tokens, topk, experts, n, k, form, int8):
+    _, args, kw, data, ref = make(tokens, topk, experts, n, k, form, int8, tokens + n)
+    check(run(args, kw, int8), *reference(*data, **ref))
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("block_size", [48, 64])
+def test_more_than_a_thousand_blocks(block_size, int8):
+    """1300 blocks and more of three experts, then the same with blocks in the
+    middle of an expert's run taken out."""
+
+    tokens, topk, experts = 21000, 4, 3
+    ids = torch.randint(0, experts, (tokens, topk), device=DEV, generator=gen(40)).to(torch.int32)
+    _, args, kw, data, ref = make(tokens, topk, experts, 288, 64, "up", int8, 41, ids=ids, block_size=block_size)
+    out = run(args, kw, int8).clone()
+    check(out, *reference(*data, **ref))
+    hurt = kw["expert_ids"].clone()
+    lost = []
+    for b in (1, 2, 700, 1023, 1024, 1100):
+        hurt[b] = -1
+        lost.append(kw["sorted_token_ids"][b * block_size:(b + 1) * block_size])
+    lost = torch.cat(lost).long()
+    lost = lost[lost < tokens * topk]
+    args[3 if int8 else 2].fill_(7.0)
+    got = run(args, {**kw, "expert_ids": hurt}, int8)
+    assert (got[lost] == 7.0).all()
+    kept = torch.ones(tokens * topk, dtype=torch.bool, device=DEV)
+    kept[lost] = False
+    assert torch.equal(got[kept], out[kept])
+
+
+def test_output_past_four_gigabytes():
+    tokens, n, k = 33000, 65536, 16
+    ids = (torch.arange(tokens, device=DEV) % 2).to(torch.int32)[:, None]
+    plan = G.make_grouped_plan(tokens, 1, 2, n, k)
+    x, w = randn((tokens, k), 50).to(BF16), randn((2, n, k), 51).to(BF16)
+    out = torch.empty(plan.output_shape, dtype=BF16, device=DEV)
+    G.grouped_linear_into(x, w, out, plan=plan, **align(ids, 2, plan.block_size))
+    one = {"per_slot": False, "swiglu": False, "route": None, "clamp": 0.0}
+    for rows in (slice(0, 50), slice(tokens // 2, tokens // 2 + 50), slice(tokens - 50, tokens)):
+        check(out[rows], *reference(x[rows], w, ids[rows], **one))
+
+
+def test_calls_on_two_streams_at_once():
+    calls = [make(t, 4, 16, 512, 528, "up", int8, 70 + i) for i, (t, int8) in
+             enumerate([(20, False), (20, True), (1500, False), (1500, True)])]
+    alone = [run(args, kw, i % 2 == 1).clone() for i, (_, args, kw, _, _) in enumerate(calls)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for turn in range(10):
+        for i, (_, args, kw, _, _) in enumerate(calls):
+            with torch.cuda.stream(streams[i]):
+                run(args, kw, i % 2 == 1)
+    torch.cuda.synchronize()
+    for i, (_, args, kw, _, _) in enumerate(calls):
+        assert torch.equal(args[3 if i % 2 else 2], alone[i])
+
+
+def test_more_blocks_and_channels_than_one_launch_of_tiles_holds():
+    """9000 blocks x 2048 channel tiles x 256 lanes: past 2^32; almost all
+    blocks lie behind the last sequence."""
+
+    tokens, n, k = 100, 65536, 8
+    ids = (torch.arange(tokens, device=DEV) % 2).to(torch.int32)[:, None]
+    plan = G.make_grouped_plan(tokens, 1, 2, n, k, block_size=8)
+    x, w = randn((tokens, k), 80).to(BF16), randn((2, n, k), 81).to(BF16)
+    a = align(ids, 2, 8)
+    out = torch.full(plan.output_shape, float("nan"), dtype=BF16, device=DEV)
+    long = torch.full((72000,), tokens, dtype=torch.int32, device=DEV)
+    long[:plan.capacity] = a["sorted_token_ids"]
+    experts = torch.zeros((9000,), dtype=torch.int32, device=DEV)
+    experts[:a["expert_ids"].numel()] = a["expert_ids"]
+    ops.grouped_gemm_into(x, w, out, tokens=tokens, topk=1, sorted_token_ids=long, expert_ids=experts,
+                          num_tokens_post_padded=a["num_tokens_post_padded"], block_size=8)
+    check(out, *reference(x, w, ids, per_slot=False, swiglu=False, route=None, clamp=0.0))

@@ -196,3 +196,15 @@ def test_side_stream_and_graph_replays():
         torch.cuda.synchronize()
         for x, w, ws, out, *_ in cases:
             assert torch.equal(out, L.int8_linear(x, w, ws)), i
+
+
+def test_more_rows_than_one_launch_of_the_quantiser_holds():
+    m = 2**25 + 7  # four rows of 64 lanes a workgroup: 2^31 lanes
+    x = torch.zeros((m, 16), dtype=BF16, device=DEV)
+    rows = torch.tensor([0, 1, 2**25 - 1, 2**25, 2**25 + 1, m - 1], device=DEV)
+    x[rows] = activations(6, 16, BF16, 5)
+    q, s = quantise(x)
+    want_q, want_s = expected_codes(x[rows])
+    assert torch.equal(q[rows], want_q) and torch.equal(s[rows], want_s)
+    assert q.count_nonzero() == want_q.count_nonzero()
+    assert (s > 0).all()
