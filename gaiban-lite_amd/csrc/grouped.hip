@@ -51,43 +51,49 @@ static void launch_grouped_tile(ProductParams p, hipStream_t stream) {
     hipLaunchKernelGGL((product_tile_kernel<Op, TOK, CH, WM, WN, WK, S, true, SWIGLU, false>), grid, block, 0, stream, p);
 }
 
-// The kernel of a call.  Blocks of up to 16 slots (few tokens): 16 x 32 tiles, 512 bytes of K
-// a stage, which stream the weights at 6.3 TB/s (64 tokens, 256 experts, N=4096, K=2048: 530
-// us against 545-575 with 64 channels and 128 bytes).  Blocks of 32: 128 channels where there
-// are workgroups enough (1000 tokens over 256 experts, N=K=4096 1556 us against 1672 with 64;
-// 60 tokens x 2 over 8 experts 60 us against 53).  Longer blocks: the least time by a model --
-// a start, then a CU's share of the tiles times (K blocks x time per block + end), or the
-// experts' weights at 5.9 TB/s where that is more; the tiles per expert are estimated from
-// the mean (the routes are on the device).  us, bf16, model / measured: 5000 tokens x 4 over
-// 64 experts, N=K=1024: 128 x 256 62 / 58, 256 x 256 63 / 65, 128 x 128 65 / 68, 64 x 128 77 /
-// 80, 64 x 64 96 / 92; 200 x 2 over 8, N=2048, K=1024: 64 x 64 8.6 / 9.2, 64 x 128 11.3 / 10.4,
-// 128 x 128 15 / 13.
+// The kernel of a call.  Blocks of up to 32 slots: 64 x 128 tiles where there are two per CU (300
+// tokens x 6 over 64 experts, N=1024, K=4096 114 us against 124 with 32 x 64; 60 x 2 over 8
+// experts, N=K=4096, one per CU, 44.8 against 42.8), but 16 x 32 tiles with 512 bytes of K a
+// stage for blocks of up to 16 (64 tokens x 6 over 256 experts, N=4096, K=2048 480 us, 7.0 TB/s,
+// against 505 with 32 x 64 and 510 with 64 x 128), unless the rows are too short for them (K=1024
+// 271 us against 237) or many experts have more than 16 slots and are read twice (500 x 6 over
+// 256 experts, int8, N=K=4096 717 us against 646).
+// Longer blocks: the least time by a model -- a start, then a CU's share of the tiles times (K
+// blocks x time per block + end), or the experts' weights at 6.4 TB/s (the workgroups that stay:
+// 5.9) where that is more, half of the second and later readings coming from the caches; the
+// tiles per expert are estimated from the mean (the routes are on the device).  us, bf16, model /
+// measured: 5000 tokens x 4 over 64 experts, N=K=1024: 128 x 256 62 / 58, 256 x 256 63 / 65, 128
+// x 128 73 / 68, 64 x 128 77 / 80, 64 x 64 96 / 92; 200 x 2 over 8, N=2048, K=1024: 64 x 64 8.6 /
+// 8.8, 64 x 128 11.3 / 10.7, 128 x 128 16 / 13; 700 x 4 over 64, N=1024, K=2048: 64 x 128 42 /
+// 47, 128 x 256 46 / 65; 1500 x 6 over 64, N=2816, K=2048 256 x 256 170 / 184, 128 x 256 180 /
+// 210, 128 x 128 186 / 238.
 template <class Op, bool SWIGLU>
 static void launch_grouped(const ProductParams& p, hipStream_t stream) {
   const double used = p.slots < p.experts ? p.slots : p.experts;
   auto tiles = [&](int tok, int ch) { return used * tiles_per_expert(p, tok) * ((p.n + ch - 1) / ch); };
-  if (p.block_size <= 16) return launch_grouped_tile<Op, 16, 32, 1, 1, 4, 2, SWIGLU>(p, stream);
   if (p.block_size <= 32) {
-    if (tiles(32, 128) >= 4 * kGemmCus) return launch_grouped_tile<Op, 32, 128, 1, 4, 2, 3, SWIGLU>(p, stream);
+    if (tiles(64, 128) >= 2 * kGemmCus && (p.block_size > 16 || p.kbytes <= 2048 || p.slots > 10 * used))
+      return launch_grouped_tile<Op, 64, 128, 2, 4, 1, 3, SWIGLU>(p, stream);
+    if (p.block_size <= 16) return launch_grouped_tile<Op, 16, 32, 1, 1, 4, 2, SWIGLU>(p, stream);
     return launch_grouped_tile<Op, 32, 64, 1, 2, 2, 3, SWIGLU>(p, stream);
   }
   struct Tile {
     int tok, ch;
-    double start, block, end;
+    double start, block, end, rate;
     void (*launch)(ProductParams, hipStream_t);
   };
   static const Tile kernels[] = {
-      {128, 256, 5.0, 1.0, 3.0, launch_grouped_gemm<Op, 128, 256, 2, 4, SWIGLU>},
-      {256, 256, 5.0, 1.62, 3.0, launch_grouped_gemm<Op, 256, 256, 4, 2, SWIGLU>},
-      {128, 128, 5.0, 0.47, 2.5, launch_grouped_gemm<Op, 128, 128, 4, 2, SWIGLU>},
-      {64, 128, 4.0, 0.38, 1.2, launch_grouped_tile<Op, 64, 128, 2, 4, 1, 3, SWIGLU>},
-      {64, 64, 4.0, 0.25, 0.6, launch_grouped_tile<Op, 64, 64, 2, 2, 1, 3, SWIGLU>},
+      {128, 256, 5.0, 1.0, 3.0, 5.9e6, launch_grouped_gemm<Op, 128, 256, 2, 4, SWIGLU>},
+      {256, 256, 5.0, 1.62, 3.0, 5.9e6, launch_grouped_gemm<Op, 256, 256, 4, 2, SWIGLU>},
+      {128, 128, 5.0, 0.55, 2.5, 5.9e6, launch_grouped_gemm<Op, 128, 128, 4, 2, SWIGLU>},
+      {64, 128, 4.0, 0.38, 1.2, 6.4e6, launch_grouped_tile<Op, 64, 128, 2, 4, 1, 3, SWIGLU>},
+      {64, 64, 4.0, 0.25, 0.6, 6.4e6, launch_grouped_tile<Op, 64, 64, 4, 2, 1, 3, SWIGLU>},
   };
-  const double read = used * p.n * p.kbytes / 5.9e6;
   const Tile* best = nullptr;
   double least = 0.0;
   for (const Tile& t : kernels) {
     const double rounds = std::ceil(tiles(t.tok, t.ch) / kGemmCus);
+    const double read = used * p.n * p.kbytes / t.rate * (0.5 + 0.5 * tiles_per_expert(p, t.tok));
     const double time = std::max(read, t.start + rounds * (p.kblocks * t.block + t.end));
     if (best == nullptr || time < least) best = &t, least = time;
   }
