@@ -412,3 +412,16 @@ def test_more_blocks_and_channels_than_one_launch_of_tiles_holds():
     ops.grouped_gemm_into(x, w, out, tokens=tokens, topk=1, sorted_token_ids=long, expert_ids=experts,
                           num_tokens_post_padded=a["num_tokens_post_padded"], block_size=8)
     check(out, *reference(x, w, ids, per_slot=False, swiglu=False, route=None, clamp=0.0))
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("tokens,topk,experts,n,k", [
+    (64, 4, 128, 2048, 512), (40, 4, 128, 1024, 1024), (40, 4, 20, 1056, 4608), (1000, 4, 128, 1024, 1024),
+    (1500, 4, 128, 1024, 1024), (3000, 4, 128, 1024, 1024), (60, 2, 8, 2048, 8192),
+])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_hundred_megabytes_of_weights(tokens, topk, experts, n, k, form, int8):
+    _, args, kw, data, ref = make(tokens, topk, experts, n, k, form, int8, tokens + n)
+    out = run(args, kw, int8).clone()
+    check(out, *reference(*data, **ref))
+    assert torch.equal(run(args, kw, int8), out)
