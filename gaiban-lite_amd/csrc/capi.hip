@@ -1,5 +1,6 @@
 // extern "C" entry points of include/dsv4moe.h: argument validation (before
 // any launch), dispatch to the kernels, and the thread-local error message.
+#include <initializer_list>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -914,6 +915,26 @@ int dsv4moe_w8a16_fp8_linear(const uint16_t* a, int64_t m, int64_t n, int64_t k,
                            static_cast<hipStream_t>(stream), 0, weight_layout == DSV4MOE_WEIGHT_ROWMAJOR);
 }
 
+// The bytes that a call writes may not be bytes that it reads or writes elsewhere.
+struct Span {
+  const char* name;
+  const void* data;
+  int64_t bytes;
+};
+static int validate_apart(const char* who, std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  auto apart = [&](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.data), y = reinterpret_cast<uintptr_t>(b.data);
+    return a.data == nullptr || b.data == nullptr || x + a.bytes <= y || y + b.bytes <= x;
+  };
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    for (auto v = written.begin(); v != w; ++v)
+      DSV4_REQUIRE(apart(*w, *v), "%s: %s and %s overlap", who, w->name, v->name);
+    for (const Span& r : read) DSV4_REQUIRE(apart(*w, r), "%s: %s and %s overlap", who, w->name, r.name);
+  }
+  return DSV4MOE_OK;
+}
+static int64_t x_bytes(int32_t x_dtype) { return x_dtype == DSV4MOE_DTYPE_FP32 ? 4 : 2; }
+
 static int validate_act_quant_int8(const char* who, const void* x, int32_t x_dtype, int64_t m, int64_t k,
                                    const int8_t* q, const float* scale) {
   DSV4_REQUIRE(x_dtype >= 0 && x_dtype <= 2, "%s: x_dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)", who);
@@ -944,7 +965,9 @@ static int validate_int8_gemm(const char* who, const void* a, const float* a_sca
 int dsv4moe_act_quant_int8(const void* x, int32_t x_dtype, int64_t m, int64_t k, int8_t* q, float* scale,
                            void* stream) {
   clear_error();
-  const int rc = validate_act_quant_int8("act_quant_int8", x, x_dtype, m, k, q, scale);
+  int rc = validate_act_quant_int8("act_quant_int8", x, x_dtype, m, k, q, scale);
+  if (rc == DSV4MOE_OK)
+    rc = validate_apart("act_quant_int8", {{"q", q, m * k}, {"scale", scale, m * 4}}, {{"x", x, m * k * x_bytes(x_dtype)}});
   if (rc != DSV4MOE_OK || m == 0) return rc;
   return dsv4_launch_act_quant_int8(x, x_dtype, m, k, q, scale, static_cast<hipStream_t>(stream));
 }
@@ -952,7 +975,10 @@ int dsv4moe_act_quant_int8(const void* x, int32_t x_dtype, int64_t m, int64_t k,
 int dsv4moe_int8_gemm(const int8_t* a, const float* a_scale, int64_t m, int64_t n, int64_t k, const int8_t* wq,
                       const uint16_t* ws, uint16_t* out, void* stream) {
   clear_error();
-  const int rc = validate_int8_gemm("int8_gemm", a, a_scale, m, n, k, wq, ws, out);
+  int rc = validate_int8_gemm("int8_gemm", a, a_scale, m, n, k, wq, ws, out);
+  if (rc == DSV4MOE_OK)
+    rc = validate_apart("int8_gemm", {{"out", out, m * n * 2}},
+                        {{"a", a, m * k}, {"a_scale", a_scale, m * 4}, {"wq", wq, n * k}, {"ws", ws, n * 2}});
   if (rc != DSV4MOE_OK || m == 0) return rc;
   return dsv4_launch_int8_gemm(a, a_scale, m, n, k, wq, ws, out, static_cast<hipStream_t>(stream));
 }
@@ -962,6 +988,9 @@ int dsv4moe_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t n, in
   clear_error();
   int rc = validate_act_quant_int8("int8_linear", x, x_dtype, m, k, q, scale);
   if (rc == DSV4MOE_OK) rc = validate_int8_gemm("int8_linear", q, scale, m, n, k, wq, ws, out);
+  if (rc == DSV4MOE_OK)
+    rc = validate_apart("int8_linear", {{"out", out, m * n * 2}, {"q", q, m * k}, {"scale", scale, m * 4}},
+                        {{"x", x, m * k * x_bytes(x_dtype)}, {"wq", wq, n * k}, {"ws", ws, n * 2}});
   if (rc != DSV4MOE_OK || m == 0) return rc;
   return dsv4_launch_int8_linear(x, x_dtype, m, n, k, wq, ws, q, scale, out, static_cast<hipStream_t>(stream));
 }
@@ -1023,15 +1052,31 @@ static int grouped_params(const char* who, bool int8, const void* x, const float
   return DSV4MOE_OK;
 }
 
+// What a call of grouped_params writes beside what it reads; x and its scales, or the storage
+// they are quantised into from `from` (bytes).
+static int grouped_apart(const char* who, const dsv4::ProductParams& p, const void* from, int64_t from_bytes) {
+  const Span out{"out", p.out, (int64_t)p.slots * p.out_n * 2}, x{"x", p.x, p.rows * p.kbytes};
+  const Span scale{"x_scale", p.x_scale, p.rows * 4};
+  const Span w{"w", p.w, (int64_t)p.experts * p.n * p.kbytes}, ws{"ws", p.w_scale, (int64_t)p.experts * p.n * 2};
+  const Span ids{"sorted_token_ids", p.sorted_ids, (int64_t)p.capacity * 4};
+  const Span experts{"expert_ids", p.expert_ids, (int64_t)p.blocks * 4};
+  const Span padded{"num_tokens_post_padded", p.post_padded, 4};
+  const Span route{"route_weights", p.route_weights, (int64_t)p.slots * 4};
+  if (from == nullptr) return validate_apart(who, {out}, {x, scale, w, ws, ids, experts, padded, route});
+  return validate_apart(who, {out, {"q", p.x, x.bytes}, {"scale", p.x_scale, scale.bytes}},
+                        {{"x", from, from_bytes}, w, ws, ids, experts, padded, route});
+}
+
 int dsv4moe_grouped_gemm(const uint16_t* x, int64_t tokens, int32_t topk, int32_t per_slot, int64_t n, int64_t k,
                          int32_t experts, const uint16_t* w, const int32_t* sorted_token_ids, int64_t capacity,
                          const int32_t* expert_ids, const int32_t* num_tokens_post_padded, int32_t block_size,
                          int32_t swiglu, float clamp_limit, const float* route_weights, uint16_t* out, void* stream) {
   clear_error();
   dsv4::ProductParams p;
-  const int rc = grouped_params("grouped_gemm", false, x, nullptr, tokens, topk, per_slot, n, k, experts, w, nullptr,
+  int rc = grouped_params("grouped_gemm", false, x, nullptr, tokens, topk, per_slot, n, k, experts, w, nullptr,
                                 sorted_token_ids, capacity, expert_ids, num_tokens_post_padded, block_size, swiglu,
                                 clamp_limit, route_weights, out, &p);
+  if (rc == DSV4MOE_OK && tokens > 0) rc = grouped_apart("grouped_gemm", p, nullptr, 0);
   if (rc != DSV4MOE_OK || tokens == 0) return rc;
   return dsv4_launch_grouped(p, false, swiglu != 0, static_cast<hipStream_t>(stream));
 }
@@ -1043,9 +1088,10 @@ int dsv4moe_grouped_int8_gemm(const int8_t* x, const float* x_scale, int64_t tok
                               float clamp_limit, const float* route_weights, uint16_t* out, void* stream) {
   clear_error();
   dsv4::ProductParams p;
-  const int rc = grouped_params("grouped_int8_gemm", true, x, x_scale, tokens, topk, per_slot, n, k, experts, w, ws,
+  int rc = grouped_params("grouped_int8_gemm", true, x, x_scale, tokens, topk, per_slot, n, k, experts, w, ws,
                                 sorted_token_ids, capacity, expert_ids, num_tokens_post_padded, block_size, swiglu,
                                 clamp_limit, route_weights, out, &p);
+  if (rc == DSV4MOE_OK && tokens > 0) rc = grouped_apart("grouped_int8_gemm", p, nullptr, 0);
   if (rc != DSV4MOE_OK || tokens == 0) return rc;
   return dsv4_launch_grouped(p, true, swiglu != 0, static_cast<hipStream_t>(stream));
 }
@@ -1062,6 +1108,7 @@ int dsv4moe_grouped_int8_linear(const void* x, int32_t x_dtype, int64_t tokens, 
   int rc = grouped_params(who, true, q, scale, tokens, topk, per_slot, n, k, experts, w, ws, sorted_token_ids, capacity,
                           expert_ids, num_tokens_post_padded, block_size, swiglu, clamp_limit, route_weights, out, &p);
   if (rc == DSV4MOE_OK) rc = validate_act_quant_int8(who, x, x_dtype, per_slot ? tokens * topk : tokens, k, q, scale);
+  if (rc == DSV4MOE_OK && tokens > 0) rc = grouped_apart(who, p, x, p.rows * k * x_bytes(x_dtype));
   if (rc != DSV4MOE_OK || tokens == 0) return rc;
   rc = dsv4_launch_act_quant_int8(x, x_dtype, p.rows, k, q, scale, static_cast<hipStream_t>(stream));
   if (rc != DSV4MOE_OK) return rc;

@@ -119,8 +119,8 @@ __device__ __forceinline__ void opaque(uint32_t& v) {
 //
 // The MFMA bounds it, at the clock that its power leaves: int8 M=8192 N=16384 K=4096 414 to 451
 // us (2.4-2.6 PTOP/s, MFMA busy 0.68 of the cycles); 8192 tokens x 6 over 256 bf16 experts, N=K=
-// 4096, where the weights are streamed as well, 1879 us (0.66).  Tiles of one K block order: with
-// first_block's the rows that tiles share miss the L2 (447 -> 462 us).
+// 4096, where the weights are streamed as well, 1879 us (0.66).  All tiles begin at
+// K = 0: in first_block's order the rows that tiles share miss the L2 (447 -> 462 us).
 template <class Op, int TOK, int CH, int WM, int WN, bool GROUPED, bool SWIGLU, bool ONCE>
 __global__ __launch_bounds__(512, 1) void product_gemm_kernel(ProductParams p) {
   constexpr int kWaves = WM * WN;

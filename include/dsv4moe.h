@@ -578,7 +578,8 @@ int dsv4moe_dequant_fp8_block(const void* w, int32_t w_dtype, const float* scale
  * dsv4moe_int8_linear: both from x.  q and scale are storage of the call: their
  *   contents afterwards are unspecified.
  * m >= 0, n % 16 == 0, k % 16 == 0, k <= 65536, n*k below 2^31; every pointer
- * 16-byte aligned except scale and a_scale (4).
+ * 16-byte aligned except scale and a_scale (4).  What a call writes overlaps nothing
+ * else of it.
  */
 int dsv4moe_act_quant_int8(const void* x, int32_t x_dtype, int64_t m, int64_t k, int8_t* q, float* scale,
                            void* stream);
@@ -612,7 +613,7 @@ int dsv4moe_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t n, in
  *   storage of the call.
  * n % 16 == 0 (32 with swiglu); k % 8 == 0 (bf16) or 16 (int8, k <= 65536); n*k and
  * x below 2^31 bytes each; pointers 16-byte aligned except x_scale, route_weights and
- * the alignment (4).
+ * the alignment (4); out (and q and scale) overlap nothing else of the call.
  */
 int dsv4moe_grouped_gemm(const uint16_t* x, int64_t tokens, int32_t topk, int32_t per_slot, int64_t n, int64_t k,
                          int32_t experts, const uint16_t* w, const int32_t* sorted_token_ids, int64_t capacity,

@@ -127,3 +127,30 @@ def test_wrong_tensors_are_refused():
         G.grouped_linear_into(gx, gw, go, **{**kw, "sorted_token_ids": ids[:-1]})
     with pytest.raises(ValueError, match="weight"):
         G.grouped_linear_into(gx, gw[:2], go, **kw)
+
+
+def at(value):
+    return ctypes.c_void_p(value)
+
+
+@pytest.mark.parametrize("out,q,scale,said", [
+    (0x10000 + 2 * 64 - 16, 0x40000, 0x50000, "out and x"), (0x20000, 0x40000, 0x50000, "out and wq"),
+    (0x30000, 0x40000, 0x50000, "out and ws"), (0x40010, 0x40000, 0x50000, "q and out"),
+    (0x60000, 0x10000, 0x50000, "q and x"), (0x60000, 0x40000, 0x4003C, "scale and q"),
+    (0x60000, 0x40000, 0x20004, "scale and wq"),
+])
+def test_int8_calls_that_overlap(out, q, scale, said):
+    args = (at(0x10000), 0, 2, 32, 32, at(0x20000), at(0x30000), at(q), at(scale), at(out), None)
+    assert said in einval("dsv4moe_int8_linear", *args)
+
+
+def test_overlaps_of_the_parts():
+    assert "q and x" in einval("dsv4moe_act_quant_int8", at(0x10000), 2, 2, 32, at(0x100F0), at(0x50000), None)
+    gemm = (at(0x10000), at(0x20000), 2, 32, 32, at(0x30000), at(0x40000), at(0x10000), None)
+    assert "out and a" in einval("dsv4moe_int8_gemm", *gemm)
+    assert "out and x" in einval("dsv4moe_grouped_gemm", *grouped_args(x=at(0x20000), out=at(0x20000), sorted_ids=FAKE))
+    assert "out and sorted_token_ids" in einval(
+        "dsv4moe_grouped_gemm", *grouped_args(x=at(0x20000), out=at(0x80000), sorted_ids=at(0x80010)))
+    linear = (at(0x10000), 0, 4, 2, 0, 64, 64, 3, at(0x20000), at(0x30000), at(0x40000), 29, at(0x41000), at(0x42000), 8,
+              0, 0.0, None, at(0x43000), at(0x50000), at(0x43010), None)
+    assert "q and out" in einval("dsv4moe_grouped_int8_linear", *linear)
