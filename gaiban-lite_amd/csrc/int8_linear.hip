@@ -160,7 +160,9 @@ static void launch_quant(const void* x, int64_t m, int k, int8_t* q, float* scal
 // of a strip needs a barrier: there the eight partial sums (exact, int32) are added.  A lane
 // whose token does not exist reads another's codes, for a column that nothing stores.
 // Weights from HBM, us, against the quantiser and a tile kernel: N=K=4096 M=1 8.0 / 13.8, M=8
-// 10.8 / 14.3, N=16384 M=1 17.3 (3.9 TB/s) / 21.6, N=4096 K=2048 M=16 9.0 / 10.1.
+// 10.8 / 14.3, N=16384 M=1 17.3 (3.9 TB/s) / 21.6, N=4096 K=2048 M=16 9.0 / 10.1.  Two copies
+// of the weights in turn: N=16384 K=4096 15.1 -> 14.2 by strips that begin at parts of K of
+// their own, N=131072 M=8 100 -> 91 (5.9 TB/s) by copies past the caches.
 struct FewParams {
   const void* x;
   int m, n, k;
@@ -182,7 +184,7 @@ __device__ __forceinline__ void lds_wait_all() {
 #endif
 }
 
-template <int X>
+template <int X, bool ONCE>
 __global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
   __shared__ __attribute__((aligned(256))) uint8_t lds[kFewWaves * kFewStages * 16 * kFewSlice];
   __shared__ __attribute__((aligned(256))) uint8_t codes[kFewCodes];  // [m][rounds * kFewRound]
@@ -204,15 +206,17 @@ __global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
       __builtin_amdgcn_make_buffer_rsrc((void*)p.w, (short)0, (int)((int64_t)p.n * p.k), kTileRsrcFlags);
   const int mine = strips > (int)blockIdx.x ? (strips - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
   const int steps = mine * rounds;  // over this workgroup's strips
+  // the part of K of a step: a strip's first differs from its neighbours' (as first_block)
+  auto round_of = [&](int step) { return (step + (blockIdx.x + step / rounds * gridDim.x) * 5) % rounds; };
   auto copy = [&](int step, int stage) {
     const int strip = blockIdx.x + step / rounds * gridDim.x;
-    const int k0 = step % rounds * kFewRound + wave * kFewSlice;
+    const int k0 = round_of(step) * kFewRound + wave * kFewSlice;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = i * 4 + copy_row;
       const int at = k0 + lds_part<kFewSlice>(row, lane & 15) * 16;
       const uint32_t off = step < steps && at < p.k ? (uint32_t)((strip * 16 + row) * p.k + at) : kTileOob;
-      lds_copy16(w_rsrc, ring + stage * 16 * kFewSlice + i * 1024, off, 0);
+      copy_weights16<ONCE>(w_rsrc, ring + stage * 16 * kFewSlice + i * 1024, off, 0);
     }
   };
 #pragma unroll
@@ -263,7 +267,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
   for (int step = 0; step < steps; ++step) {
     lds_dma_wait_keep<(kFewStages - 2) * 4>();
     const uint8_t* ws = lds + (wave * kFewStages + stage) * 16 * kFewSlice;
-    const uint8_t* xs = my_codes + step % rounds * kFewRound;
+    const uint8_t* xs = my_codes + round_of(step) * kFewRound;
     u32x4 wf[4], xf[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
@@ -307,8 +311,12 @@ __global__ __launch_bounds__(512) void int8_few_kernel(FewParams p) {
 template <int X>
 static int launch_few(const FewParams& p, hipStream_t stream) {
   const int strips = p.n / 16;
-  hipLaunchKernelGGL((int8_few_kernel<X>), dim3((unsigned)(strips < kGemmCus ? strips : kGemmCus)), dim3(512), 0,
-                     stream, p);
+  const dim3 grid((unsigned)(strips < kGemmCus ? strips : kGemmCus));
+  // weights that the cache in front of HBM would not hold until the next call bypass it
+  if (p.k % 128 == 0 && (int64_t)p.n * p.k > 96000000)
+    hipLaunchKernelGGL((int8_few_kernel<X, true>), grid, dim3(512), 0, stream, p);
+  else
+    hipLaunchKernelGGL((int8_few_kernel<X, false>), grid, dim3(512), 0, stream, p);
   DSV4_CHECK_LAUNCH("int8_few_kernel");
   return DSV4MOE_OK;
 }

@@ -208,3 +208,11 @@ def test_more_rows_than_one_launch_of_the_quantiser_holds():
     assert torch.equal(q[rows], want_q) and torch.equal(s[rows], want_s)
     assert q.count_nonzero() == want_q.count_nonzero()
     assert (s > 0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 24592, 4096), (5, 24592, 4224), (16, 98320, 1024), (3, 7696, 14336)])
+def test_few_tokens_over_a_hundred_megabytes(m, n, k):
+    x = activations(m, k, BF16, m + n)
+    w, ws = weights(n, k, m + k)
+    q, s = expected_codes(x)
+    assert torch.equal(L.int8_linear(x, w, ws), expected(q, s, w, ws))
